@@ -187,6 +187,104 @@ int bpt_decode_kivi_partial(const bpt_kivi_cache* cache,
                             int batch, int q_heads, int max_blocks, float scale, int splits,
                             float* o_part, float* lse, unsigned* status, void* stream);
 
+/* ---------------------------------------------------------------- scored decode, eviction
+ *
+ * Decode attention that scores the cached tokens, the append that starts their state, and the
+ * eviction that keeps the best of them (no reference counterpart). A token's state is kept by
+ * (sequence, kv head, logical slot): scores [B, Hkv, T] fp32 and positions [B, Hkv, T] int32,
+ * inner stride 1, other strides free, T the slots that a sequence can have. Evicted caches hold
+ * a sequence's tokens out of order (attention does not depend on it), so a slot's position is
+ * recorded; next_pos [B] is the position that the sequence's next token will have.
+ * Each sequence that is appended to or compacted must own its pages alone. */
+enum bpt_dtype { BPT_FP16 = 1, BPT_BF16 = 2 };
+
+/* Arguments of bpt_decode_scored. Strides in elements, inner strides 1.
+ * maps 1, the scored decode: q [B, Hq, D], caches [num_blocks, block_size, Hkv, D], out
+ *   [B, Hq, D]; Hq / Hkv <= 8; D 64, 128 or 256. q head j reads kv head j / (Hq / Hkv).
+ *   score[b, h, t] = decay * score + sum over the head's q heads of their weight of token t.
+ * maps 2, the differential decode: q [B, 2 H, D], k_cache [.., 2 Hkv, D], v_cache
+ *   [.., Hkv, 2 D], out [B, H, 2 D]; H / Hkv <= 4; D 64 or 128. q_heads is 2 H. Output head j is
+ *   (softmax(q_2j.k_2h) - lam_j softmax(q_2j+1.k_2h+1)) v_h, h = j / (H / Hkv); where norm_weight
+ *   [2 D] is set it is divided by sqrt(mean square + norm_eps) and multiplied by the weight;
+ *   then by out_scale. The score adds the sum of |weight of map 1 - lam_j weight of map 2|.
+ * q, caches and out are fp16 or bf16; scores, lam and norm_weight fp32. Softmax, sums and
+ * scores are fp32. An empty sequence gives zeros. decay 0 ignores the old scores (NaN among
+ * them); slots past a sequence's end keep theirs. Keys must be finite with maps 2. */
+typedef struct bpt_scored_decode {
+  int dtype, maps;
+  int batch, q_heads, kv_heads, head_dim, block_size, max_blocks;
+  int num_splits, sm_count;                          /* as bpt_decode_fp16 */
+  float scale, decay, norm_eps, out_scale;           /* scale <= 0: 1 / sqrt(head_dim) */
+  int64_t num_blocks;
+  const void* q;        int64_t q_stride[2];         /* batch, head */
+  const void* k_cache;  int64_t k_stride[3];         /* block, token, head */
+  const void* v_cache;  int64_t v_stride[3];
+  const int32_t* block_table;  int64_t bt_stride;
+  const int32_t* seq_lens;
+  void* out;            int64_t out_stride[2];       /* batch, head */
+  float* scores;        int64_t scores_stride[2];    /* nullable; batch, head; T >= all slots */
+  const float* lam;     int64_t lam_stride[2];       /* maps 2: batch (0: shared), head */
+  const float* norm_weight;                          /* nullable, maps 2 */
+} bpt_scored_decode;
+
+/* Split count and workspace of bpt_decode_scored. tokens: max_blocks * block_size with scores,
+ * 0 without. The workspace starts with the status word and must be 16-byte aligned. */
+int bpt_effective_splits_scored(int head_dim, int maps, int batch, int kv_heads, int block_size,
+                                int max_blocks, int num_splits, int sm_count);
+size_t bpt_scored_workspace_bytes(int head_dim, int maps, int batch, int q_heads, int splits,
+                                  int64_t tokens);
+int bpt_decode_scored(const bpt_scored_decode* args, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* A 16-bit paged cache that is written: k [num_blocks, block_size, k_heads, k_dim] and v
+ * [num_blocks, block_size, v_heads, v_dim], strides in elements, inner strides 1. block_size a
+ * power of two up to 256. */
+typedef struct bpt_paged_cache {
+  int block_size, k_heads, v_heads, k_dim, v_dim;
+  int64_t num_blocks;
+  void* k;  int64_t k_stride[3];                     /* block, token, head */
+  void* v;  int64_t v_stride[3];
+} bpt_paged_cache;
+
+/* Write tokens t < new_lens[b] of k_new [B, max_new, k_heads, k_dim] / v_new (strides batch,
+ * token, head) to slots seq_lens[b] + t. Where given, scores of the new slots become 0 and
+ * positions next_pos[b] + t, for v_heads heads (T >= max_blocks * block_size). Tokens past the
+ * table, and tokens of a page outside the cache, are not written and flagged in *status
+ * (nullable). Nothing else is touched: the caller advances seq_lens. */
+int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new, const int64_t* kn_stride,
+                      const void* v_new, const int64_t* vn_stride, const int32_t* new_lens,
+                      const int32_t* seq_lens, const int32_t* block_table, int64_t bt_sb,
+                      int max_blocks, int batch, int max_new, float* scores, int64_t sc_sb,
+                      int64_t sc_sh, int32_t* positions, int64_t pos_sb, int64_t pos_sh,
+                      const int32_t* next_pos, unsigned* status, void* stream);
+
+/* Most moves that an eviction of rows of `slots` slots can need (at least 1). */
+int bpt_evict_moves(int budget, int slots);
+
+/* Choose `budget` slots of every (sequence, kv head) of more than budget tokens: first those
+ * with position < sinks or position >= next_pos - recent, then the highest scores (NaN lowest),
+ * ties to the lowest slot. src / dst [B, Hkv, bpt_evict_moves(budget, slots)] contiguous
+ * receive the moves that bring them to slots < budget: the i-th evicted slot below budget, in
+ * ascending order, takes the i-th kept slot at or past it, in descending order; -1 past
+ * counts[b, h]. new_lens[b] = min(seq_lens[b], budget) (not seq_lens itself). Lengths are
+ * clamped to [0, slots]. Needs recent + sinks <= budget. */
+int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t sc_sh,
+                         const int32_t* positions, int64_t pos_sb, int64_t pos_sh,
+                         const int32_t* seq_lens, const int32_t* next_pos, int batch,
+                         int kv_heads, int slots, int budget, int recent, int sinks,
+                         int32_t* src, int32_t* dst, int32_t* counts, int32_t* new_lens,
+                         void* stream);
+
+/* Carry out moves: rows src -> dst (slots) of k, v and, where given, of scores and positions
+ * with `slots` slots a row. k_heads and v_heads must be equal; a differential cache's pairs of
+ * key heads are one head of twice the width. Moves outside the table, the state rows or the
+ * cache are skipped and flagged in *status (nullable). */
+int bpt_compact_cache(const bpt_paged_cache* cache, const int32_t* block_table, int64_t bt_sb,
+                      int max_blocks, const int32_t* src, const int32_t* dst,
+                      const int32_t* counts, int moves, int batch, float* scores, int64_t sc_sb,
+                      int64_t sc_sh, int32_t* positions, int64_t pos_sb, int64_t pos_sh,
+                      int slots, unsigned* status, void* stream);
+
 /* Size of the fixed scratch array behind bpt_decode_fp16_noalloc, per GPU. */
 #define BPT_NOALLOC_SCRATCH_BYTES (8u * 1024u * 1024u)
 

@@ -28,6 +28,10 @@ struct DecodeParams {
   int balance;      // 1: splits sized by the batch's longest sequence (split_range)
   int64_t num_blocks;
   float scale_log2; // softmax scale * log2(e)
+  // the split kernels of the scored and the differential decode only (mma::OpState)
+  float* part_l;       // [B, Hq, S] sums of the partials; lse then holds their maxima (log2)
+  float* logits;       // nullable: [B, Hq, logit_pitch] scaled logits (log2), tokens < n written
+  int64_t logit_pitch; // a multiple of the chunk's tokens
 };
 
 struct WorkspaceView {

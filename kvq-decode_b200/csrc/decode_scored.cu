@@ -1,0 +1,451 @@
+// Decode attention that says what the cached tokens were worth: the scored decode and the
+// differential decode over a paged fp16 / bf16 cache. No reference counterpart.
+//
+//   scored  x_gt = scale q_g.k_t, p_gt = exp(x_gt - max_t x) / sum_t exp(..)  (t < n)
+//           out_g = sum_t p_gt v_t;  score_t <- decay * score_t + sum_g p_gt
+//   diff    output head j has two q heads, two key heads and one value head of twice the width:
+//           a_jt = p1_jt - lam_j p2_jt;  o_j = sum_t a_jt v_t;  with a norm weight
+//           o_j <- o_j / sqrt(mean(o_j^2) + eps) * w;  out_j = out_scale * o_j
+//           score_t <- decay * score_t + sum_j |a_jt|
+//
+// Two launches. The split kernel (mma_decode.cuh, OpState) is the fp16 decode's: one CTA per
+// (sequence, kv head, split) reads K and V once for all the rows of the head. It also leaves
+// every token's scaled logit in the workspace (4 bytes per row and token). A token's weight
+// needs the sum over the whole sequence, known only when every split has ended, so the second
+// kernel forms it: per row the splits' (max, sum) are joined, then 2^(x - M) / L of every token
+// is added to its score, while other CTAs of the same launch join the splits' outputs. The
+// logits cost 8 bytes a row and token (written and read, mostly in the 126 MB L2) where
+// reading the keys again would cost 2 D a kv head and token.
+#include <cuda_bf16.h>
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "decode_common.h"
+#include "mma_decode.cuh"
+
+namespace bpt {
+namespace {
+
+constexpr float kNegInf = -INFINITY;
+constexpr int kFinishThreads = 256;
+constexpr int kFinishWarps = kFinishThreads / 32;
+constexpr int kScoreTokens = 4 * kFinishThreads;  // tokens of one scoring CTA
+constexpr int kMaxRows = 8;                       // q rows per kv head
+
+// Split CTA shape by (concatenated key) width: as the fp16 decode's.
+template <int D>
+struct Shape {
+  static constexpr int NCW = D >= 256 ? 4 : 2;
+  static constexpr int STAGES = D >= 256 ? 2 : 3;
+  static constexpr int MINB = D >= 256 ? 1 : 4;
+};
+
+int chunk_tokens(int width) { return width >= 256 ? 16 * Shape<256>::NCW : 16 * Shape<128>::NCW; }
+int resident_ctas(int width) { return width >= 256 ? Shape<256>::MINB : Shape<128>::MINB; }
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+struct FinishParams {
+  const float* m;       // [B, R, S] maxima (log2), R = rows per sequence
+  const float* l;       // [B, R, S] sums
+  const float* o_part;  // [B, R, S, D] normalised partial outputs
+  const float* logits;  // [B, R, pitch]
+  int64_t pitch;
+  const int32_t* seq_lens;
+  int64_t cap;
+  float* scores;
+  int64_t sc_sb, sc_sh;
+  float decay;
+  int score_vec;        // score rows are 16-byte aligned
+  const float* lam;
+  int64_t lam_sb, lam_sh;
+  const float* norm_w;  // nullable, [D]
+  float norm_eps, out_scale;
+  void* out;
+  int64_t o_sb, o_sh;
+  int kv_heads, group, splits;
+  int n_merge;          // CTAs [0, n_merge) join outputs, the others score tokens
+  int out_heads, chunks;
+};
+
+// (M, 1 / L) of one row over its S splits; every lane gets it. L = 0 (no token) gives 0.
+__device__ __forceinline__ void row_state(const float* m, const float* l, int S, int lane,
+                                          float& M, float& inv) {
+  float mx = kNegInf, sum = 0.f;
+  for (int s = lane; s < S; s += 32) {
+    const float ms = m[s], ls = l[s];
+    const float mn = fmaxf(mx, ms);
+    if (mn != kNegInf) {
+      sum = sum * fast_exp2(mx - mn) + ls * fast_exp2(ms - mn);
+      mx = mn;
+    } else {
+      sum += ls;   // 0, or NaN of a NaN logit
+    }
+  }
+  M = mx;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(kFullMask, M, o));
+  if (M == kNegInf) M = 0.f;
+  float L = sum * fast_exp2(mx - M);
+  if (mx == kNegInf) L = sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(kFullMask, L, o);
+  inv = L == 0.f ? 0.f : 1.f / L;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store16(void* base, int64_t at, float x) {
+  if constexpr (BF16)
+    static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(x);
+  else
+    static_cast<__half*>(base)[at] = __float2half_rn(x);
+}
+
+// One output row (b, j): sum over its maps and splits of sign * (share of the split) * o.
+template <int D, bool BF16, bool DIFF>
+__device__ __forceinline__ void join_output(const FinishParams& p, int id, float* s_o,
+                                            float* s_red) {
+  constexpr int MAPS = DIFF ? 2 : 1;
+  constexpr int V4 = (D + 127) / 128;             // float4 columns of a lane
+  constexpr int U = 4;                            // rows in flight
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = id / p.out_heads, j = id % p.out_heads;
+  const int S = p.splits;
+  float4 acc[V4];
+#pragma unroll
+  for (int v = 0; v < V4; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int map = 0; map < MAPS; ++map) {
+    const int64_t row = (int64_t(b) * p.out_heads + j) * MAPS + map;
+    const float* m = p.m + row * S;
+    const float* l = p.l + row * S;
+    const float* o = p.o_part + row * S * D;
+    float M, inv;
+    row_state(m, l, S, lane, M, inv);
+    if (DIFF && map == 1) inv *= -p.lam[int64_t(b) * p.lam_sb + int64_t(j) * p.lam_sh];
+    for (int s0 = warp; s0 < S; s0 += kFinishWarps * U) {
+      float f[U];
+      float4 x[U][V4];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + kFinishWarps * u;
+        const bool in = s < S;
+        const float ls = in ? l[s] : 0.f;
+        f[u] = ls == 0.f ? 0.f : fast_exp2(m[in ? s : 0] - M) * ls * inv;
+#pragma unroll
+        for (int v = 0; v < V4; ++v) {
+          const int c = 4 * (32 * v + lane);
+          x[u][v] = (in && c < D) ? *reinterpret_cast<const float4*>(o + int64_t(s) * D + c)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int v = 0; v < V4; ++v) {
+          acc[v].x = fmaf(f[u], x[u][v].x, acc[v].x);
+          acc[v].y = fmaf(f[u], x[u][v].y, acc[v].y);
+          acc[v].z = fmaf(f[u], x[u][v].z, acc[v].z);
+          acc[v].w = fmaf(f[u], x[u][v].w, acc[v].w);
+        }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V4; ++v) {
+    const int c = 4 * (32 * v + lane);
+    if (c < D) *reinterpret_cast<float4*>(s_o + warp * D + c) = acc[v];
+  }
+  __syncthreads();
+  float r = 0.f;
+  if (tid < D) {
+#pragma unroll
+    for (int w = 0; w < kFinishWarps; ++w) r += s_o[w * D + tid];
+  }
+  float mul = p.out_scale;
+  if (DIFF && p.norm_w) {                         // uniform over the CTA
+    float sq = r * r;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(kFullMask, sq, o);
+    if (lane == 0) s_red[warp] = sq;
+    __syncthreads();
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFinishWarps; ++w) total += s_red[w];
+    mul *= rsqrtf(total / float(D) + p.norm_eps);
+    if (tid < D) mul *= p.norm_w[tid];
+  }
+  if (tid < D)
+    store16<BF16>(p.out, int64_t(b) * p.o_sb + int64_t(j) * p.o_sh + tid, DIFF ? r * mul : r);
+}
+
+// kScoreTokens tokens of one (sequence, kv head).
+template <bool DIFF>
+__device__ __forceinline__ void score_tokens(const FinishParams& p, int id, float* s_m,
+                                             float* s_inv, float* s_lam) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int chunk = id % p.chunks, bh = id / p.chunks;
+  const int b = bh / p.kv_heads, h = bh % p.kv_heads;
+  const int n = int(min(int64_t(max(p.seq_lens[b], 0)), p.cap));
+  const int64_t t0 = int64_t(chunk) * kScoreTokens;
+  if (t0 >= n) return;                            // uniform over the CTA
+  const int G = p.group;
+  const int64_t row0 = int64_t(bh) * G;
+  const int64_t t = t0 + 4 * tid;
+  // the logits are asked for before the splits' states: their latencies overlap
+  float4 x[kMaxRows];
+#pragma unroll
+  for (int r = 0; r < kMaxRows; ++r)
+    if (r < G && t < n) x[r] = *reinterpret_cast<const float4*>(p.logits + (row0 + r) * p.pitch + t);
+  if (warp < G) {
+    float M, inv;
+    row_state(p.m + (row0 + warp) * p.splits, p.l + (row0 + warp) * p.splits, p.splits, lane, M,
+              inv);
+    if (lane == 0) {
+      s_m[warp] = M;
+      s_inv[warp] = inv;
+      if (DIFF)
+        s_lam[warp] = p.lam[int64_t(b) * p.lam_sb + int64_t((h * G + warp) >> 1) * p.lam_sh];
+    }
+  }
+  __syncthreads();
+  if (t >= n) return;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  float a[4];
+#pragma unroll
+  for (int r = 0; r < kMaxRows; ++r)
+    if (r < G) {
+      const float M = s_m[r], inv = s_inv[r];
+      const float e[4] = {fast_exp2(x[r].x - M) * inv, fast_exp2(x[r].y - M) * inv,
+                          fast_exp2(x[r].z - M) * inv, fast_exp2(x[r].w - M) * inv};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!DIFF) w[i] += e[i];
+        else if ((r & 1) == 0) a[i] = e[i];
+        else w[i] += fabsf(a[i] - s_lam[r] * e[i]);
+      }
+    }
+  float* sc = p.scores + int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh + t;
+  if (p.score_vec && t + 4 <= n) {
+    float4 o = make_float4(w[0], w[1], w[2], w[3]);
+    if (p.decay != 0.f) {
+      const float4 old = *reinterpret_cast<const float4*>(sc);
+      o.x = fmaf(p.decay, old.x, w[0]);
+      o.y = fmaf(p.decay, old.y, w[1]);
+      o.z = fmaf(p.decay, old.z, w[2]);
+      o.w = fmaf(p.decay, old.w, w[3]);
+    }
+    *reinterpret_cast<float4*>(sc) = o;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t + i < n) sc[i] = p.decay != 0.f ? fmaf(p.decay, sc[i], w[i]) : w[i];
+}
+
+template <int D, bool BF16, bool DIFF>
+__global__ void __launch_bounds__(kFinishThreads)
+finish_scored_kernel(const FinishParams p) {
+  __shared__ __align__(16) float s_o[kFinishWarps * D];
+  __shared__ float s_a[kMaxRows], s_b[kMaxRows], s_c[kMaxRows];
+  pdl_wait();
+  // the next call's split kernel may start launching; it waits for this grid's end
+  pdl_launch_dependents();
+  if (int(blockIdx.x) < p.n_merge)
+    join_output<D, BF16, DIFF>(p, blockIdx.x, s_o, s_a);
+  else
+    score_tokens<DIFF>(p, int(blockIdx.x) - p.n_merge, s_a, s_b, s_c);
+}
+
+template <int D, bool BF16, bool DIFF>
+int launch_both(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p,
+                const FinishParams& f, cudaStream_t st) {
+  using S = Shape<D>;
+  using Op = mma::OpState<BF16, DIFF>;
+  const int rc = p.group > 4
+                     ? mma::launch<D, S::NCW, S::STAGES, S::MINB, true, Op>(tk, tv, p, st)
+                     : mma::launch<D, S::NCW, S::STAGES, S::MINB, false, Op>(tk, tv, p, st);
+  if (rc) return rc;
+  const int64_t grid = int64_t(f.n_merge) +
+                       (f.scores ? int64_t(p.batch) * p.kv_heads * f.chunks : 0);
+  return launch_dependent(finish_scored_kernel<D, BF16, DIFF>, dim3(unsigned(grid)),
+                          dim3(kFinishThreads), 0, st, f) == cudaSuccess
+             ? BPT_OK
+             : BPT_ERR_LAUNCH;
+}
+
+template <int D, bool DIFF>
+int launch_typed(bool bf16, const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p,
+                 const FinishParams& f, cudaStream_t st) {
+  return bf16 ? launch_both<D, true, DIFF>(tk, tv, p, f, st)
+              : launch_both<D, false, DIFF>(tk, tv, p, f, st);
+}
+
+int64_t logit_pitch(int64_t cap) { return (cap + 63) / 64 * 64; }   // whole chunks, 16 bytes
+
+struct ScoredView {
+  unsigned* status;
+  float *m, *l, *o_part, *logits;
+  size_t bytes;
+};
+
+// [status word, padded][maxima][sums][partial outputs][logits], each padded to 256 bytes
+ScoredView scored_view(void* ws, int batch, int rows, int width, int splits, int64_t tokens) {
+  char* base = static_cast<char*>(ws);
+  const size_t n = size_t(batch) * rows * splits;
+  const size_t state = align256(n * sizeof(float));
+  const size_t part = align256(n * width * sizeof(float));
+  ScoredView v;
+  v.status = reinterpret_cast<unsigned*>(base);
+  v.m = reinterpret_cast<float*>(base + 256);
+  v.l = reinterpret_cast<float*>(base + 256 + state);
+  v.o_part = reinterpret_cast<float*>(base + 256 + 2 * state);
+  v.logits = reinterpret_cast<float*>(base + 256 + 2 * state + part);
+  v.bytes = 256 + 2 * state + part +
+            (tokens > 0 ? size_t(batch) * rows * logit_pitch(tokens) * sizeof(float) : 0);
+  return v;
+}
+
+int state_splits(int width, int batch, int kv_heads, int block_size, int max_blocks,
+                 int num_splits, int sm_count) {
+  const int chunk = chunk_tokens(width);
+  const int s = num_splits > 0 ? num_splits
+                               : plan_splits(batch, kv_heads, block_size, max_blocks, sm_count,
+                                             resident_ctas(width), chunk);
+  return clamp_splits(s, block_size, max_blocks, chunk);
+}
+
+bool misaligned(const void* x, int bytes) { return reinterpret_cast<uintptr_t>(x) % bytes; }
+
+}  // namespace
+}  // namespace bpt
+
+using namespace bpt;
+
+extern "C" int bpt_effective_splits_scored(int head_dim, int maps, int batch, int kv_heads,
+                                           int block_size, int max_blocks, int num_splits,
+                                           int sm_count) {
+  return state_splits(maps * head_dim, batch, kv_heads, block_size, max_blocks, num_splits,
+                      sm_count);
+}
+
+extern "C" size_t bpt_scored_workspace_bytes(int head_dim, int maps, int batch, int q_heads,
+                                             int splits, int64_t tokens) {
+  if (batch <= 0 || q_heads <= 0 || head_dim <= 0 || splits <= 0 || maps <= 0) return 256;
+  return scored_view(nullptr, batch, q_heads, maps * head_dim, splits, tokens).bytes;
+}
+
+extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  if (!a) return BPT_ERR_INVALID_ARGUMENT;
+  const int maps = a->maps;
+  if ((maps != 1 && maps != 2) || (a->dtype != BPT_FP16 && a->dtype != BPT_BF16))
+    return BPT_ERR_INVALID_ARGUMENT;
+  if (a->batch < 0 || a->kv_heads <= 0 || a->q_heads <= 0 || a->q_heads % (maps * a->kv_heads) ||
+      a->block_size <= 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->head_dim <= 0)
+    return BPT_ERR_INVALID_ARGUMENT;
+  if (a->batch == 0) return BPT_OK;
+  if (!a->q || !a->k_cache || !a->v_cache || (!a->block_table && a->max_blocks > 0) ||
+      !a->seq_lens || !a->out || !workspace || (maps == 2 && !a->lam))
+    return BPT_ERR_INVALID_ARGUMENT;
+  const int D = a->head_dim, width = maps * D;
+  const int group = a->q_heads / a->kv_heads;
+  if (group > kMaxRows) return BPT_ERR_UNSUPPORTED_SHAPE;
+  if (!(width == 64 || width == 128 || width == 256) || D < 64) return BPT_ERR_UNSUPPORTED_SHAPE;
+  if (a->block_size < 16 || a->block_size > 256 || (a->block_size & (a->block_size - 1)))
+    return BPT_ERR_UNSUPPORTED_SHAPE;
+  // q fragments are read as 4-byte pairs; outputs are single elements; the tensor maps check
+  // the caches
+  if (misaligned(a->q, 4) || a->q_stride[0] % 2 || a->q_stride[1] % 2) return BPT_ERR_ALIGNMENT;
+  const int64_t cap = int64_t(a->max_blocks) * a->block_size;
+  if (cap > INT32_MAX) return BPT_ERR_UNSUPPORTED_SHAPE;
+  const int S = state_splits(width, a->batch, a->kv_heads, a->block_size, a->max_blocks,
+                             a->num_splits, a->sm_count);
+  const int64_t tokens = a->scores ? cap : 0;
+  const ScoredView ws = scored_view(workspace, a->batch, a->q_heads, width, S, tokens);
+  if (workspace_bytes < ws.bytes) return BPT_ERR_WORKSPACE_TOO_SMALL;
+  if (misaligned(workspace, 16)) return BPT_ERR_ALIGNMENT;
+
+  DecodeParams p{};
+  const int chunk = chunk_tokens(width);
+  const int box_rows = a->block_size < chunk ? a->block_size : chunk;
+  const CUtensorMapDataType type = a->dtype == BPT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tk, tv;
+  int rc = encode_kv_map(&tk, a->k_cache, type, 2, D, maps * a->kv_heads, a->block_size,
+                         a->num_blocks, a->k_stride[2], a->k_stride[1], a->k_stride[0], 64,
+                         box_rows, &p.k_c1, 128);
+  if (rc) return rc;
+  rc = encode_kv_map(&tv, a->v_cache, type, 2, width, a->kv_heads, a->block_size, a->num_blocks,
+                     a->v_stride[2], a->v_stride[1], a->v_stride[0], 64, box_rows, &p.v_c1, 128);
+  if (rc) return rc;
+  p.q = static_cast<const __half*>(a->q);   // 16-bit elements, read as pairs
+  p.q_sb = a->q_stride[0];
+  p.q_sh = a->q_stride[1];
+  p.block_table = a->block_table;
+  p.bt_sb = a->bt_stride;
+  p.seq_lens = a->seq_lens;
+  p.o_part = ws.o_part;
+  p.lse = ws.m;
+  p.part_l = ws.l;
+  p.logits = a->scores ? ws.logits : nullptr;
+  p.logit_pitch = logit_pitch(cap);
+  p.status = ws.status;
+  p.batch = a->batch;
+  p.q_heads = a->q_heads;
+  p.kv_heads = a->kv_heads;
+  p.group = group;
+  p.splits = S;
+  p.final_out = 0;
+  p.balance = balanced_splits(a->batch, a->kv_heads, S, resident_ctas(width)) ? 1 : 0;
+  p.block_size = a->block_size;
+  p.max_blocks = a->max_blocks;
+  p.box_rows = box_rows;
+  p.num_blocks = a->num_blocks;
+  const float sc = a->scale > 0.f ? a->scale : 1.0f / sqrtf(float(D));
+  p.scale_log2 = sc * 1.4426950408889634f;
+
+  FinishParams f{};
+  f.m = ws.m;
+  f.l = ws.l;
+  f.o_part = ws.o_part;
+  f.logits = ws.logits;
+  f.pitch = p.logit_pitch;
+  f.seq_lens = a->seq_lens;
+  f.cap = cap;
+  f.scores = a->scores;
+  f.sc_sb = a->scores_stride[0];
+  f.sc_sh = a->scores_stride[1];
+  f.decay = a->decay;
+  f.score_vec = !misaligned(a->scores, 16) && f.sc_sb % 4 == 0 && f.sc_sh % 4 == 0;
+  f.lam = a->lam;
+  f.lam_sb = a->lam_stride[0];
+  f.lam_sh = a->lam_stride[1];
+  f.norm_w = a->norm_weight;
+  f.norm_eps = a->norm_eps;
+  f.out_scale = a->out_scale;
+  f.out = a->out;
+  f.o_sb = a->out_stride[0];
+  f.o_sh = a->out_stride[1];
+  f.kv_heads = a->kv_heads;
+  f.group = group;
+  f.splits = S;
+  f.out_heads = a->q_heads / maps;
+  f.n_merge = a->batch * f.out_heads;
+  f.chunks = int((cap + kScoreTokens - 1) / kScoreTokens);
+  if (int64_t(f.n_merge) + int64_t(a->batch) * a->kv_heads * f.chunks > INT32_MAX)
+    return BPT_ERR_UNSUPPORTED_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf16 = a->dtype == BPT_BF16;
+  if (maps == 2)
+    rc = D == 64 ? launch_typed<128, true>(bf16, tk, tv, p, f, st)
+                 : launch_typed<256, true>(bf16, tk, tv, p, f, st);
+  else if (D == 64)
+    rc = launch_typed<64, false>(bf16, tk, tv, p, f, st);
+  else if (D == 128)
+    rc = launch_typed<128, false>(bf16, tk, tv, p, f, st);
+  else
+    rc = launch_typed<256, false>(bf16, tk, tv, p, f, st);
+  if (rc) return rc;
+  return cudaGetLastError() == cudaSuccess ? BPT_OK : BPT_ERR_LAUNCH;
+}

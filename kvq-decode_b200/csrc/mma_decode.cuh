@@ -23,7 +23,18 @@
 // K/V stage buffers are 64-column blocks written by TMA with the 128-byte swizzle (16-byte
 // chunk c of token row r lands at chunk c ^ (r % 8)); every ldmatrix phase then reads 8
 // distinct bank groups.
+//
+// The last template parameter says what an instance reads and leaves behind. OpFp16 is the
+// fp16 decode. OpState<BF16, DIFF> serves the scored and the differential decode: its splits
+// leave (max, sum) apart instead of their log-sum-exp, and, where DecodeParams::logits is set,
+// every token's scaled logit. DIFF pairs two key heads with one value head of twice their
+// width: a q row of map 0 is followed by zeros, one of map 1 preceded by them, so that one
+// product over the concatenated keys gives both maps' logits and every K and V byte is still
+// read once (half of the Q.K^T products are with zeros; the kernel is bound by the cache's
+// bytes).
 #pragma once
+
+#include <cuda_bf16.h>
 
 #include "common.cuh"
 #include "split_state.cuh"
@@ -34,7 +45,16 @@ namespace mma {
 
 constexpr float kNegInf = -INFINITY;
 
-template <int D, int NCW, int STAGES, bool G8>
+struct OpFp16 {
+  static constexpr bool kBf16 = false, kState = false, kDiff = false;
+};
+
+template <bool BF16, bool DIFF>
+struct OpState {
+  static constexpr bool kBf16 = BF16, kState = true, kDiff = DIFF;
+};
+
+template <int D, int NCW, int STAGES, bool G8, typename Op = OpFp16>
 struct Cfg {
   static constexpr int CHUNK = 16 * NCW;              // tokens per stage
   static constexpr int THREADS = (NCW + 1) * 32;      // + 1 producer warp
@@ -44,7 +64,7 @@ struct Cfg {
   static constexpr int STAGE_ELEMS = CHUNK * D;
   static constexpr int KSTEPS = D / 16;
   static constexpr int DB16 = D / 16;                 // 16-row d blocks of O^T
-  static constexpr int NACC = G8 ? 2 : 1;
+  static constexpr int NACC = G8 && !Op::kState ? 2 : 1;
   static constexpr size_t MERGE_BYTES = size_t(NCW) * 8 * (D + 3) * 4;
   static constexpr size_t RING_BYTES = size_t(STAGES) * STAGE_ELEMS * 2 * 2;
   static constexpr size_t BODY_BYTES = RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES;
@@ -65,35 +85,54 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint3
                : "r"(addr));
 }
 
+template <bool BF16 = false>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                           uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
 }
 
 // d = A.B with a zero accumulator (a fresh partial product).
+template <bool BF16 = false>
 __device__ __forceinline__ void mma_16816_zc(float (&d)[4], uint32_t a0, uint32_t a1,
                                              uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  if constexpr (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  }
 }
 
 // acc += A.B, with the product formed by the tensor core from a zero accumulator and added
 // in fp32 round-to-nearest: a long-running accumulator never passes through the tensor
 // core's own accumulation, whose per-step rounding would otherwise build up over thousands
 // of tokens on a large running sum.
+template <bool BF16 = false>
 __device__ __forceinline__ void mma_16816_acc(float (&acc)[4], uint32_t a0, uint32_t a1,
                                               uint32_t a2, uint32_t a3, uint32_t b0,
                                               uint32_t b1) {
   float t[4];
-  mma_16816_zc(t, a0, a1, a2, a3, b0, b1);
+  mma_16816_zc<BF16>(t, a0, a1, a2, a3, b0, b1);
   acc[0] += t[0]; acc[1] += t[1]; acc[2] += t[2]; acc[3] += t[3];
 }
 
@@ -102,8 +141,19 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// fp16 hi = fp16(p) and lo = fp16(p - hi) for two adjacent tokens, packed as half2.
+// hi = fp16(p) and lo = fp16(p - hi) for two adjacent tokens, packed as half2: ~22 bits of p.
+// With bf16 (whose MMA takes bf16 operands only) the pair carries ~16 bits, a relative error
+// of at most 2^-17 in a weight whose output is rounded to bf16 (2^-9).
+template <bool BF16 = false>
 __device__ __forceinline__ void split_hi_lo(float p0, float p1, uint32_t& hi, uint32_t& lo) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+    const float2 hf = __bfloat1622float2(h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(p0 - hf.x, p1 - hf.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    return;
+  }
   __half2 h = __floats2half2_rn(p0, p1);
   const float2 hf = __half22float2(h);
   hi = *reinterpret_cast<uint32_t*>(&h);
@@ -114,11 +164,11 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-template <int D, int NCW, int STAGES, int MINB, bool G8>
+template <int D, int NCW, int STAGES, int MINB, bool G8, typename Op = OpFp16>
 __global__ void __launch_bounds__((NCW + 1) * 32, MINB)
 split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const DecodeParams p) {
-  using C = Cfg<D, NCW, STAGES, G8>;
+  using C = Cfg<D, NCW, STAGES, G8, Op>;
   constexpr int CHUNK = C::CHUNK;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -173,7 +223,10 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       } else {
         const int64_t row = (int64_t(b) * p.q_heads + qh0 + g) * S + split;
         p.o_part[row * D + d] = 0.f;
-        if (d == 0) p.lse[row] = kNegInf;
+        if (d == 0) {
+          p.lse[row] = kNegInf;
+          if constexpr (Op::kState) p.part_l[row] = 0.f;
+        }
       }
     }
     return;
@@ -232,8 +285,11 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
 #pragma unroll
           for (int cb = 0; cb < C::NCB; ++cb) {
             const int so = stage * C::STAGE_ELEMS + cb * C::BLOCK_ELEMS + j * R * 64;
-            tma_load_4d(sK + so, &tmK, &full[stage], cb * 64, p.k_c1 ? row : h,
-                        p.k_c1 ? h : row, phys, pol);
+            // DIFF: the first half of the columns is key head 2h, the second key head 2h + 1
+            const int kcol = Op::kDiff ? cb * 64 % (D / 2) : cb * 64;
+            const int kh = Op::kDiff ? 2 * h + cb * 64 / (D / 2) : h;
+            tma_load_4d(sK + so, &tmK, &full[stage], kcol, p.k_c1 ? row : kh,
+                        p.k_c1 ? kh : row, phys, pol);
             tma_load_4d(sV + so, &tmV, &full[stage], cb * 64, p.v_c1 ? row : h,
                         p.v_c1 ? h : row, phys, pol);
           }
@@ -263,8 +319,12 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
         p.q + int64_t(b) * p.q_sb + int64_t(qh0 + (qvalid ? qhead : 0)) * p.q_sh;
 #pragma unroll
     for (int ks = 0; ks < C::KSTEPS; ++ks) {
-      qa0[ks] = qvalid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * t4) : 0u;
-      qa2[ks] = qvalid ? *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * t4) : 0u;
+      // DIFF: row r is map r & 1 of output head r >> 1; its q meets its own half of the keys
+      constexpr int kHalf = C::KSTEPS / 2;
+      const bool on = Op::kDiff ? qvalid && (qhead & 1) == ks / kHalf : qvalid;
+      const int col = 16 * (Op::kDiff ? ks % kHalf : ks) + 2 * t4;
+      qa0[ks] = on ? *reinterpret_cast<const uint32_t*>(qrow + col) : 0u;
+      qa2[ks] = on ? *reinterpret_cast<const uint32_t*>(qrow + col + 8) : 0u;
     }
   }
 
@@ -309,8 +369,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       const uint32_t addr = kbase + uint32_t(ks >> 2) * C::BLOCK_BYTES + ld_row + (chunk << 4);
       uint32_t b0, b1, b2, b3;
       ldsm_x4(addr, b0, b1, b2, b3);
-      mma_16816(s0, qa0[ks], 0u, qa2[ks], 0u, b0, b1);
-      mma_16816(s1, qa0[ks], 0u, qa2[ks], 0u, b2, b3);
+      mma_16816<Op::kBf16>(s0, qa0[ks], 0u, qa2[ks], 0u, b0, b1);
+      mma_16816<Op::kBf16>(s1, qa0[ks], 0u, qa2[ks], 0u, b2, b3);
     }
 
     // ---- online softmax (log2 domain): this lane owns q head `qhead`, tokens 2t, 2t+1, +8
@@ -319,6 +379,16 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     const float x1 = (tk + 1 < lim) ? s0[1] * sl2 : kNegInf;
     const float x2 = (tk + 8 < lim) ? s1[0] * sl2 : kNegInf;
     const float x3 = (tk + 9 < lim) ? s1[1] * sl2 : kNegInf;
+    if constexpr (Op::kState) {
+      // 8-byte stores: the 4 lanes of a row fill whole 32-byte sectors. A row's pitch covers
+      // whole chunks, so the tokens past lim land in its own padding.
+      if (p.logits && qvalid && (G8 || g < 4)) {
+        float* row = p.logits + (int64_t(b) * p.q_heads + qh0 + qhead) * p.logit_pitch +
+                     (u0 + c) * CHUNK + warp * 16 + tk;
+        *reinterpret_cast<float2*>(row) = make_float2(x0, x1);
+        *reinterpret_cast<float2*>(row + 8) = make_float2(x2, x3);
+      }
+    }
     float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
     mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2));
@@ -341,8 +411,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     const float p2 = fast_exp2(x2 - m_use), p3 = fast_exp2(x3 - m_use);
     l_run += (p0 + p1) + (p2 + p3);
     uint32_t hi0, lo0, hi1, lo1;
-    split_hi_lo(p0, p1, hi0, lo0);
-    split_hi_lo(p2, p3, hi1, lo1);
+    split_hi_lo<Op::kBf16>(p0, p1, hi0, lo0);
+    split_hi_lo<Op::kBf16>(p2, p3, hi1, lo1);
 
     // ---- rows past the end of the split: zero V so stale or NaN bytes cannot reach O
     if (lim < 16) {
@@ -365,8 +435,19 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       const uint32_t addr = vbase + uint32_t(db >> 2) * C::BLOCK_BYTES + ld_row + (chunk << 4);
       uint32_t a0, a1, a2, a3;
       ldsm_x4_trans(addr, a0, a1, a2, a3);
-      mma_16816_acc(acc[0][db], a0, a1, a2, a3, pb0, pb1);
-      if constexpr (G8) mma_16816_acc(acc[C::NACC - 1][db], a0, a1, a2, a3, lo0, lo1);
+      if constexpr (G8 && Op::kState) {
+        // hi and lo products of one tile meet in the tensor core, the tiles in fp32: half of
+        // the accumulator registers (168 + spills against none at D = 128)
+        float t[4];
+        mma_16816_zc<Op::kBf16>(t, a0, a1, a2, a3, hi0, hi1);
+        mma_16816<Op::kBf16>(t, a0, a1, a2, a3, lo0, lo1);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][db][e] += t[e];
+        continue;
+      }
+      mma_16816_acc<Op::kBf16>(acc[0][db], a0, a1, a2, a3, pb0, pb1);
+      if constexpr (G8)
+        mma_16816_acc<Op::kBf16>(acc[C::NACC - 1][db], a0, a1, a2, a3, lo0, lo1);
     }
     if (lim < 16) fence_proxy_async_smem();
     __syncwarp();
@@ -384,7 +465,7 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (G8) {
-        acc[0][i][e] += acc[C::NACC - 1][i][e];
+        if constexpr (C::NACC == 2) acc[0][i][e] += acc[C::NACC - 1][i][e];
       } else {
         acc[0][i][e] += __shfl_xor_sync(kFullMask, acc[0][i][e], 2);
       }
@@ -405,16 +486,16 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     }
   }
   named_barrier_sync(1, NCW * 32);
-  write_split_state<NCW, D>(sM, sL, sAcc, sAcc + NCW * 8 * D, p, b, qh0, split,
-                            int(threadIdx.x), NCW * 32,
-                            [] { named_barrier_sync(1, NCW * 32); });
+  write_split_state<NCW, D, Op::kState>(sM, sL, sAcc, sAcc + NCW * 8 * D, p, b, qh0, split,
+                                        int(threadIdx.x), NCW * 32,
+                                        [] { named_barrier_sync(1, NCW * 32); });
 }
 
-template <int D, int NCW, int STAGES, int MINB, bool G8>
+template <int D, int NCW, int STAGES, int MINB, bool G8, typename Op = OpFp16>
 int launch(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p,
            cudaStream_t st) {
-  using C = Cfg<D, NCW, STAGES, G8>;
-  auto kern = split_kv_fp16_mma_kernel<D, NCW, STAGES, MINB, G8>;
+  using C = Cfg<D, NCW, STAGES, G8, Op>;
+  auto kern = split_kv_fp16_mma_kernel<D, NCW, STAGES, MINB, G8, Op>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(C::SMEM_BYTES)) != cudaSuccess)
     return BPT_ERR_LAUNCH;

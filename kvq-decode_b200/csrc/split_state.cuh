@@ -19,7 +19,10 @@ namespace bpt {
 // element is then one fma chain and one vector store per 4 channels: the epilogue of the split
 // that ends last is on the call's critical path, while the SM's other CTAs still stream, and
 // the per-element form (max, exp2 and a division for every element) took ~1.7 us there.
-template <int NW, int D, typename Sync>
+// STATE: the split's (max, sum) go to p.lse and p.part_l apart. A weight formed from a rounded
+// log-sum-exp would be off by half a step of the exponent (2^-21 at a logit of 8), more than
+// the rest of the weight's fp32 arithmetic.
+template <int NW, int D, bool STATE = false, typename Sync>
 __device__ __forceinline__ void write_split_state(const float* sM, const float* sL,
                                                   const float* sAcc, float* sF,
                                                   const DecodeParams& p, int b, int qh0,
@@ -41,9 +44,14 @@ __device__ __forceinline__ void write_split_state(const float* sM, const float* 
     const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) sF[hg * NW + w] = f[w] * inv;
-    if (!to_out)
+    if constexpr (STATE) {
+      const int64_t row = (int64_t(b) * p.q_heads + qh0 + hg) * S + split;
+      p.lse[row] = M;
+      p.part_l[row] = L;
+    } else if (!to_out) {
       p.lse[(int64_t(b) * p.q_heads + qh0 + hg) * S + split] =
           L > 0.f ? M + __log2f(L) : kNegInfS;
+    }
   }
   sync();
   // caller partial buffers may be offset views: vector stores only where aligned
