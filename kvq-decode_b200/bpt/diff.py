@@ -54,17 +54,8 @@ def paged_decode_attention_diff(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     the sum over its output heads: the weight by which the token's value counts. An empty
     sequence gives zeros. No host synchronisation.
     """
-    _require(q.dim() == 3 and q.shape[1] % 2 == 0, "q must be [B, 2 H, D]")
-    B, H, D = q.shape[0], q.shape[1] // 2, q.shape[2]
-    _require(lam is not None and lam.dtype == torch.float32 and
-             (lam.shape == (H,) or lam.shape == (B, H)), f"lam must be float32 [{H}] or [{B}, {H}]")
-    if norm_weight is not None:
-        _require(norm_weight.shape == (2 * D,) and norm_weight.dtype == torch.float32 and
-                 norm_weight.is_contiguous(), f"norm_weight must be contiguous float32 [{2 * D}]")
-        _require(norm_eps >= 0.0, "norm_eps must not be negative")
     return _decode_scored(2, q, k_cache, v_cache, block_table, seq_lens, scale, num_splits, scores,
-                          float(decay), out, workspace, lam, norm_weight, float(norm_eps),
-                          float(out_scale))
+                          decay, out, workspace, lam, norm_weight, norm_eps, out_scale)
 
 
 __all__ = ["paged_decode_attention_diff", "diff_lambda"]

@@ -3,10 +3,12 @@
     python kvq-decode_b200/build.py [--force] [--verbose]
 
 Compiles every ``csrc/*.cu`` for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``)
-with nvcc and links one shared library exporting the C ABI declared in ``include/bpt.h``.
+with nvcc and links one shared library exporting the C ABI declared in ``include/bpt.h``, and
+``csrc/bind.cpp`` with the host compiler against torch's headers as the extension module
+``bpt/_bind`` (the Python binding of the scored decode and the eviction).
 The CUDA runtime is linked statically; the driver API is reached through
 ``cudaGetDriverEntryPointByVersion`` so the library has no link-time libcuda dependency.
-Rebuilds only when a source or header is newer than the library.
+Rebuilds only when a source or header is newer than what was built.
 """
 import argparse
 import glob
@@ -14,11 +16,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "bpt", "libbpt_b200.so")
+BIND_SRC = os.path.join(CSRC, "bind.cpp")
+BIND_OUT = os.path.join(PKG, "bpt", "_bind" + sysconfig.get_config_var("EXT_SUFFIX"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr",
          "-Xptxas", "-O3"]
@@ -41,16 +46,54 @@ def deps():
             glob.glob(os.path.join(ROOT, "include", "*.h")) + [os.path.abspath(__file__)])
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(OUT):
+def newer(out, sources_) -> bool:
+    """Whether ``out`` exists and no source is newer."""
+    if not os.path.exists(out):
         return False
-    t = os.path.getmtime(OUT)
-    return all(os.path.getmtime(d) <= t for d in deps())
+    t = os.path.getmtime(out)
+    return all(os.path.getmtime(d) <= t for d in sources_)
+
+
+def up_to_date() -> bool:
+    return newer(OUT, deps())
+
+
+def bind_up_to_date() -> bool:
+    return newer(BIND_OUT, [BIND_SRC, os.path.join(ROOT, "include", "bpt.h"),
+                            os.path.abspath(__file__)])
+
+
+def start_bind(verbose: bool):
+    """Compile and link ``bpt/_bind``; returns the running compiler."""
+    import torch
+    from torch.utils import cpp_extension
+    inc = [os.path.join(ROOT, "include"), sysconfig.get_paths()["include"],
+           *cpp_extension.include_paths(),
+           os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           *[f"-isystem{i}" for i in inc], BIND_SRC, "-o", BIND_OUT + ".tmp", "-L" + libs,
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd))
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> str:
-    if not force and up_to_date():
-        return OUT
+    bind = None if not force and bind_up_to_date() else start_bind(verbose)
+    if force or not up_to_date():
+        build_library(verbose, extra)
+    if bind is not None:
+        out, _ = bind.communicate()
+        if bind.returncode != 0:
+            raise RuntimeError(f"{BIND_SRC} failed:\n{out}")
+        os.replace(BIND_OUT + ".tmp", BIND_OUT)
+    return OUT
+
+
+def build_library(verbose: bool, extra) -> None:
     objdir = os.path.join(PKG, "_build")
     os.makedirs(objdir, exist_ok=True)
     objs = []
@@ -81,7 +124,6 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> str:
         print(" ".join(link))
     subprocess.run(link, check=True)
     os.replace(tmp, OUT)
-    return OUT
 
 
 def main():

@@ -28,21 +28,19 @@ namespace bpt {
 namespace {
 
 constexpr float kNegInf = -INFINITY;
-constexpr int kFinishThreads = 256;
-constexpr int kFinishWarps = kFinishThreads / 32;
-constexpr int kScoreTokens = 4 * kFinishThreads;  // tokens of one scoring CTA
+constexpr int kMapWarps = 8;                      // warps that join one map's splits
+constexpr int finish_threads(int maps) { return maps * kMapWarps * 32; }
+constexpr int score_tokens_of(int maps) { return 4 * finish_threads(maps); }  // of one CTA
 constexpr int kMaxRows = 8;                       // q rows per kv head
 
-// Split CTA shape by (concatenated key) width: as the fp16 decode's.
-template <int D>
-struct Shape {
-  static constexpr int NCW = D >= 256 ? 4 : 2;
-  static constexpr int STAGES = D >= 256 ? 2 : 3;
-  static constexpr int MINB = D >= 256 ? 1 : 4;
-};
-
-int chunk_tokens(int width) { return width >= 256 ? 16 * Shape<256>::NCW : 16 * Shape<128>::NCW; }
-int resident_ctas(int width) { return width >= 256 ? Shape<256>::MINB : Shape<128>::MINB; }
+// Split CTA shape: 2 warps of 16 tokens each, a 3-stage ring, and as many CTAs an SM as the ring
+// of a width allows (4 at 128 channels, 2 at 256). Width 256 measured with 64-token chunks in 2
+// stages and 1 CTA: 107 us; 32-token chunks, 3 CTAs of 2 stages (registers spill): 100 us; 2 CTAs
+// of 3 stages: 84 us (differential, B=8, 16k tokens, 4 value heads of 256).
+constexpr int kSplitWarps = 2;
+constexpr int kStages = 3;
+constexpr int kChunk = 16 * kSplitWarps;
+constexpr int resident_ctas(int width) { return width >= 256 ? 2 : 4; }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -102,53 +100,58 @@ __device__ __forceinline__ void store16(void* base, int64_t at, float x) {
     static_cast<__half*>(base)[at] = __float2half_rn(x);
 }
 
-// One output row (b, j): sum over its maps and splits of sign * (share of the split) * o.
+// One output row (b, j): sum over its maps and splits of sign * (share of the split) * o. Warps
+// 8 k .. 8 k + 7 join map k; the first U rows of a warp are asked for before the row's
+// state, so that up to 8 U splits cost one memory round trip.
 template <int D, bool BF16, bool DIFF>
 __device__ __forceinline__ void join_output(const FinishParams& p, int id, float* s_o,
                                             float* s_red) {
   constexpr int MAPS = DIFF ? 2 : 1;
+  constexpr int WARPS = MAPS * kMapWarps;
   constexpr int V4 = (D + 127) / 128;             // float4 columns of a lane
-  constexpr int U = 4;                            // rows in flight
+  constexpr int U = V4 == 1 ? 8 : 4;              // rows in flight
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int map = warp / kMapWarps, w0 = warp % kMapWarps;
   const int b = id / p.out_heads, j = id % p.out_heads;
   const int S = p.splits;
+  const int64_t row = (int64_t(b) * p.out_heads + j) * MAPS + map;
+  const float* m = p.m + row * S;
+  const float* l = p.l + row * S;
+  const float* o = p.o_part + row * S * D;
   float4 acc[V4];
 #pragma unroll
   for (int v = 0; v < V4; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = 0.f, inv = 0.f;
+  for (int s0 = w0; s0 < S; s0 += kMapWarps * U) {
+    float ms[U], ls[U];
+    float4 x[U][V4];
 #pragma unroll
-  for (int map = 0; map < MAPS; ++map) {
-    const int64_t row = (int64_t(b) * p.out_heads + j) * MAPS + map;
-    const float* m = p.m + row * S;
-    const float* l = p.l + row * S;
-    const float* o = p.o_part + row * S * D;
-    float M, inv;
-    row_state(m, l, S, lane, M, inv);
-    if (DIFF && map == 1) inv *= -p.lam[int64_t(b) * p.lam_sb + int64_t(j) * p.lam_sh];
-    for (int s0 = warp; s0 < S; s0 += kFinishWarps * U) {
-      float f[U];
-      float4 x[U][V4];
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + kMapWarps * u;
+      const bool in = s < S;
+      ms[u] = in ? m[s] : 0.f;
+      ls[u] = in ? l[s] : 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int s = s0 + kFinishWarps * u;
-        const bool in = s < S;
-        const float ls = in ? l[s] : 0.f;
-        f[u] = ls == 0.f ? 0.f : fast_exp2(m[in ? s : 0] - M) * ls * inv;
-#pragma unroll
-        for (int v = 0; v < V4; ++v) {
-          const int c = 4 * (32 * v + lane);
-          x[u][v] = (in && c < D) ? *reinterpret_cast<const float4*>(o + int64_t(s) * D + c)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+      for (int v = 0; v < V4; ++v) {
+        const int c = 4 * (32 * v + lane);
+        x[u][v] = (in && c < D) ? *reinterpret_cast<const float4*>(o + int64_t(s) * D + c)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
       }
+    }
+    if (s0 == w0) {
+      row_state(m, l, S, lane, M, inv);
+      if (DIFF && map == 1) inv *= -p.lam[int64_t(b) * p.lam_sb + int64_t(j) * p.lam_sh];
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const float f = ls[u] == 0.f ? 0.f : fast_exp2(ms[u] - M) * ls[u] * inv;
 #pragma unroll
-        for (int v = 0; v < V4; ++v) {
-          acc[v].x = fmaf(f[u], x[u][v].x, acc[v].x);
-          acc[v].y = fmaf(f[u], x[u][v].y, acc[v].y);
-          acc[v].z = fmaf(f[u], x[u][v].z, acc[v].z);
-          acc[v].w = fmaf(f[u], x[u][v].w, acc[v].w);
-        }
+      for (int v = 0; v < V4; ++v) {
+        acc[v].x = fmaf(f, x[u][v].x, acc[v].x);
+        acc[v].y = fmaf(f, x[u][v].y, acc[v].y);
+        acc[v].z = fmaf(f, x[u][v].z, acc[v].z);
+        acc[v].w = fmaf(f, x[u][v].w, acc[v].w);
+      }
     }
   }
 #pragma unroll
@@ -160,10 +163,11 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
   float r = 0.f;
   if (tid < D) {
 #pragma unroll
-    for (int w = 0; w < kFinishWarps; ++w) r += s_o[w * D + tid];
+    for (int w = 0; w < WARPS; ++w) r += s_o[w * D + tid];
   }
   float mul = p.out_scale;
   if (DIFF && p.norm_w) {                         // uniform over the CTA
+    const float w = tid < D ? p.norm_w[tid] : 0.f;
     float sq = r * r;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(kFullMask, sq, o);
@@ -171,15 +175,14 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
     __syncthreads();
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFinishWarps; ++w) total += s_red[w];
-    mul *= rsqrtf(total / float(D) + p.norm_eps);
-    if (tid < D) mul *= p.norm_w[tid];
+    for (int k = 0; k < D / 32; ++k) total += s_red[k];
+    mul *= rsqrtf(total / float(D) + p.norm_eps) * w;
   }
   if (tid < D)
     store16<BF16>(p.out, int64_t(b) * p.o_sb + int64_t(j) * p.o_sh + tid, DIFF ? r * mul : r);
 }
 
-// kScoreTokens tokens of one (sequence, kv head).
+// One CTA's tokens of one (sequence, kv head), 4 a thread.
 template <bool DIFF>
 __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, float* s_m,
                                              float* s_inv, float* s_lam) {
@@ -187,7 +190,7 @@ __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, floa
   const int chunk = id % p.chunks, bh = id / p.chunks;
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
   const int n = int(min(int64_t(max(p.seq_lens[b], 0)), p.cap));
-  const int64_t t0 = int64_t(chunk) * kScoreTokens;
+  const int64_t t0 = int64_t(chunk) * score_tokens_of(DIFF ? 2 : 1);
   if (t0 >= n) return;                            // uniform over the CTA
   const int G = p.group;
   const int64_t row0 = int64_t(bh) * G;
@@ -244,10 +247,10 @@ __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, floa
 }
 
 template <int D, bool BF16, bool DIFF>
-__global__ void __launch_bounds__(kFinishThreads)
+__global__ void __launch_bounds__(finish_threads(DIFF ? 2 : 1))
 finish_scored_kernel(const FinishParams p) {
-  __shared__ __align__(16) float s_o[kFinishWarps * D];
-  __shared__ float s_a[kMaxRows], s_b[kMaxRows], s_c[kMaxRows];
+  __shared__ __align__(16) float s_o[(DIFF ? 2 : 1) * kMapWarps * D];
+  __shared__ float s_a[2 * kMapWarps], s_b[kMaxRows], s_c[kMaxRows];
   pdl_wait();
   // the next call's split kernel may start launching; it waits for this grid's end
   pdl_launch_dependents();
@@ -260,16 +263,16 @@ finish_scored_kernel(const FinishParams p) {
 template <int D, bool BF16, bool DIFF>
 int launch_both(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p,
                 const FinishParams& f, cudaStream_t st) {
-  using S = Shape<D>;
+  constexpr int R = resident_ctas(D);
   using Op = mma::OpState<BF16, DIFF>;
   const int rc = p.group > 4
-                     ? mma::launch<D, S::NCW, S::STAGES, S::MINB, true, Op>(tk, tv, p, st)
-                     : mma::launch<D, S::NCW, S::STAGES, S::MINB, false, Op>(tk, tv, p, st);
+                     ? mma::launch<D, kSplitWarps, kStages, R, true, Op>(tk, tv, p, st)
+                     : mma::launch<D, kSplitWarps, kStages, R, false, Op>(tk, tv, p, st);
   if (rc) return rc;
   const int64_t grid = int64_t(f.n_merge) +
                        (f.scores ? int64_t(p.batch) * p.kv_heads * f.chunks : 0);
   return launch_dependent(finish_scored_kernel<D, BF16, DIFF>, dim3(unsigned(grid)),
-                          dim3(kFinishThreads), 0, st, f) == cudaSuccess
+                          dim3(finish_threads(DIFF ? 2 : 1)), 0, st, f) == cudaSuccess
              ? BPT_OK
              : BPT_ERR_LAUNCH;
 }
@@ -308,11 +311,10 @@ ScoredView scored_view(void* ws, int batch, int rows, int width, int splits, int
 
 int state_splits(int width, int batch, int kv_heads, int block_size, int max_blocks,
                  int num_splits, int sm_count) {
-  const int chunk = chunk_tokens(width);
   const int s = num_splits > 0 ? num_splits
                                : plan_splits(batch, kv_heads, block_size, max_blocks, sm_count,
-                                             resident_ctas(width), chunk);
-  return clamp_splits(s, block_size, max_blocks, chunk);
+                                             resident_ctas(width), kChunk);
+  return clamp_splits(s, block_size, max_blocks, kChunk);
 }
 
 bool misaligned(const void* x, int bytes) { return reinterpret_cast<uintptr_t>(x) % bytes; }
@@ -367,8 +369,7 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   if (misaligned(workspace, 16)) return BPT_ERR_ALIGNMENT;
 
   DecodeParams p{};
-  const int chunk = chunk_tokens(width);
-  const int box_rows = a->block_size < chunk ? a->block_size : chunk;
+  const int box_rows = a->block_size < kChunk ? a->block_size : kChunk;
   const CUtensorMapDataType type = a->dtype == BPT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tk, tv;
@@ -432,7 +433,7 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   f.splits = S;
   f.out_heads = a->q_heads / maps;
   f.n_merge = a->batch * f.out_heads;
-  f.chunks = int((cap + kScoreTokens - 1) / kScoreTokens);
+  f.chunks = int((cap + score_tokens_of(maps) - 1) / score_tokens_of(maps));
   if (int64_t(f.n_merge) + int64_t(a->batch) * a->kv_heads * f.chunks > INT32_MAX)
     return BPT_ERR_UNSUPPORTED_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -22,19 +22,22 @@ namespace {
 // ------------------------------------------------------------------------------- selection
 //
 // The budget-th largest key of a row is found by a radix select over the scores' bits, mapped
-// to unsigned keys of the same order: three passes over 11 + 11 + 10 bits, each a histogram of
-// the keys that share the digits found so far. One cluster of C CTAs takes one (sequence, kv
-// head): each CTA reads its slice of the scores and positions once and keeps the keys in shared
-// memory; histograms and prefix counts are exchanged through distributed shared memory. Ties
-// at the threshold go to the lowest slots, so the result is unique and does not depend on the
-// order in which the histogram's integer atomics arrive.
+// to unsigned keys of the same order: passes over 11 + 11 + 10 bits, each a histogram of the
+// keys that share the digits found so far, and no further pass once a bin is taken whole. One
+// cluster of C CTAs takes one (sequence, kv head). Each CTA reads its slice of the scores and
+// positions once and keeps the keys in registers (TILES of 4 a thread; longer slices are read
+// again in each pass); histograms and prefix counts are exchanged through distributed shared
+// memory. Ties at the threshold go to the lowest slots, so the result is unique and does not
+// depend on the order in which the histogram's integer atomics arrive.
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kTile = 128;                   // slots of one vector load of a warp
-constexpr int kMaxKeys = 48 * 1024;          // keys a CTA holds in shared memory (192 KB)
+constexpr int kTile = 128;                   // slots that a warp takes at a time, 4 a lane
+constexpr int kMaxTiles = 16;                // tiles of a warp that stay in registers
+constexpr int kMaxCluster = 8;
 constexpr uint32_t kProtectedKey = 0xffffffffu;
+constexpr uint32_t kNoKey = 0u;              // past the end; a score's key is at least 1
 
 struct SelectParams {
   const float* scores;
@@ -48,23 +51,40 @@ struct SelectParams {
   int moves;
   int32_t* counts;                           // [B, H]
   int32_t* new_lens;                         // [B]
-  int key_cap;                               // keys that fit the launch's shared memory
   int vec;                                   // rows are 16-byte aligned
 };
 
 // Unsigned key of the same order as the score: NaN lowest, -0 equal to +0.
 __device__ __forceinline__ uint32_t score_key(float f) {
-  if (f != f) return 0u;
   const uint32_t u = __float_as_uint(f + 0.f);
-  return u ^ ((u & 0x80000000u) ? 0xffffffffu : 0x80000000u);
+  return f != f ? 1u : u ^ ((u & 0x80000000u) ? 0xffffffffu : 0x80000000u);
 }
 
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(kFullMask, x, o);
+    if (lane >= o) x += up;
+  }
+  return x;
+}
+
+// Sum of v over the warps below this one: every lane reads one warp's v.
+__device__ __forceinline__ uint32_t below_this_warp(const uint32_t* v, int warp, int lane) {
+  uint32_t x = lane < warp ? v[lane] : 0u;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o);
+  return x;
+}
+
+template <int TILES>
 __global__ void __launch_bounds__(kSelThreads)
 select_kernel(const SelectParams p) {
-  extern __shared__ __align__(16) uint32_t smem_sel[];
-  uint32_t* s_keys = smem_sel + 2 * kBins;   // two histograms first
+  static_assert(kSelWarps <= 32, "one lane per warp in the block-wide sums");
+  static_assert(kBins == 4 * kSelThreads, "4 bins a thread");
+  __shared__ __align__(16) uint32_t s_hist[2][kBins];
   __shared__ uint32_t s_scan[kSelWarps];
-  __shared__ uint32_t s_digit, s_left;
+  __shared__ uint32_t s_digit, s_left, s_bin;
   __shared__ uint32_t s_gt[kSelWarps], s_eq[kSelWarps];
   __shared__ uint32_t s_tot[2];              // this CTA's keys above and at the threshold
 
@@ -74,13 +94,19 @@ select_kernel(const SelectParams p) {
   const int row = int(blockIdx.x) / C;
   const int b = row / p.kv_heads, h = row % p.kv_heads;
 
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    *reinterpret_cast<uint4*>(&s_hist[i][4 * tid]) = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
   const int n = min(max(p.seq_lens[b], 0), p.slots);
+  // 64-bit: next_pos - recent may pass the int range
+  const int64_t first_recent = int64_t(p.next_pos[b]) - p.recent;
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = min(n, p.budget);
   int32_t* src = p.src + int64_t(row) * p.moves;
   int32_t* dst = p.dst + int64_t(row) * p.moves;
-  // unused places; the cluster barriers below order this before the moves of any CTA
+  // unused places; the barriers of the passes order this before the moves of any CTA
   for (int i = rank * kSelThreads + tid; i < p.moves; i += C * kSelThreads) {
     src[i] = -1;
     dst[i] = -1;
@@ -90,167 +116,197 @@ select_kernel(const SelectParams p) {
     return;
   }
 
-  // this CTA's slots [lo, hi) and this warp's [w_lo, w_hi) of them: whole tiles
+  // this CTA's slots, and this warp's [w_lo, w_hi) of them: whole tiles
   const int per = cdiv(cdiv(n, C), kTile) * kTile;
   const int lo = min(n, rank * per), hi = min(n, lo + per);
   const int w_per = cdiv(cdiv(per, kSelWarps), kTile) * kTile;
   const int w_lo = min(hi, lo + warp * w_per), w_hi = min(hi, w_lo + w_per);
   const float* sc = p.scores + int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh;
   const int32_t* pos = p.positions + int64_t(b) * p.pos_sb + int64_t(h) * p.pos_sh;
-  // 64-bit: next_pos - recent may pass the int range
-  const int64_t first_recent = int64_t(p.next_pos[b]) - p.recent;
   const int32_t sinks = p.sinks;
   auto key_of = [&](float f, int32_t at) {
     return (at < sinks || at >= first_recent) ? kProtectedKey : score_key(f);
   };
-  const bool resident = per <= p.key_cap;    // else every pass reads the row again
-  auto key_at = [&](int i) { return resident ? s_keys[i - lo] : key_of(sc[i], pos[i]); };
-
-  for (int i = tid; i < 2 * kBins; i += kSelThreads) smem_sel[i] = 0u;
-  if (resident) {
-    if (p.vec) {
-#pragma unroll 4
-      for (int i = w_lo + 4 * lane; i < w_hi; i += kTile) {
-        // rows are T long: the last vector may reach past n, within the row or not
-        if (i + 4 <= w_hi) {
-          const float4 f = *reinterpret_cast<const float4*>(sc + i);
-          const int4 at = *reinterpret_cast<const int4*>(pos + i);
-          *reinterpret_cast<uint4*>(s_keys + (i - lo)) =
-              make_uint4(key_of(f.x, at.x), key_of(f.y, at.y), key_of(f.z, at.z),
-                         key_of(f.w, at.w));
-        } else {
-          for (int e = i; e < w_hi; ++e) s_keys[e - lo] = key_of(sc[e], pos[e]);
-        }
-      }
+  // keys of slots i .. i + 3 of the row
+  auto read4 = [&](int i, uint32_t (&k)[4]) {
+    if (p.vec && i + 4 <= w_hi) {
+      const float4 f = *reinterpret_cast<const float4*>(sc + i);
+      const int4 at = *reinterpret_cast<const int4*>(pos + i);
+      k[0] = key_of(f.x, at.x);
+      k[1] = key_of(f.y, at.y);
+      k[2] = key_of(f.z, at.z);
+      k[3] = key_of(f.w, at.w);
     } else {
-#pragma unroll 4
-      for (int i = w_lo + lane; i < w_hi; i += 32) s_keys[i - lo] = key_of(sc[i], pos[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k[e] = i + e < w_hi ? key_of(sc[i + e], pos[i + e]) : kNoKey;
     }
+  };
+  uint32_t held[TILES > 0 ? TILES : 1][4];
+  // f(first slot of this lane, its 4 keys) for every tile of the warp, in order
+  auto each_tile = [&](auto&& f) {
+    if constexpr (TILES > 0) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+        if (w_lo + t * kTile < w_hi) f(w_lo + t * kTile + 4 * lane, held[t]);
+    } else {
+      for (int i0 = w_lo; i0 < w_hi; i0 += kTile) {
+        uint32_t k[4];
+        read4(i0 + 4 * lane, k);
+        f(i0 + 4 * lane, k);
+      }
+    }
+  };
+  if constexpr (TILES > 0) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+      if (w_lo + t * kTile < w_hi) read4(w_lo + t * kTile + 4 * lane, held[t]);
   }
-  __syncthreads();
 
-  // ---- the threshold key and how many keys equal to it are kept
-  uint32_t prefix = 0u, mask = 0u, left = uint32_t(p.budget);
+  // ---- the threshold: keys whose masked bits are above thr are kept, of those equal to it the
+  // first `need`
+  uint32_t thr = 0u, mask = 0u, need = uint32_t(p.budget);
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t dmask = pass == 2 ? 1023u : 2047u;
-    uint32_t* hist = smem_sel + (pass & 1) * kBins;
+    uint32_t* hist = s_hist[pass & 1];
     if (pass == 2) {
       // its readers of pass 0 have passed the barrier of pass 1
-      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0u;
+      *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0u, 0u, 0u, 0u);
       __syncthreads();
     }
-    for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-      const int i = i0 + lane;
-      const uint32_t k = i < w_hi ? key_at(i) : 0u;
-      const bool in = i < w_hi && (k & mask) == prefix;
-      // the protected tokens come in long runs of one key: one atomic for the warp's
-      const unsigned run = __ballot_sync(kFullMask, in && k == kProtectedKey);
-      if (in && k != kProtectedKey) atomicAdd(hist + ((k >> shift) & dmask), 1u);
-      if (run && lane == 0) atomicAdd(hist + dmask, uint32_t(__popc(run)));
+    uint32_t safe = 0u;
+    each_tile([&](int, const uint32_t (&k)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (k[e] == kProtectedKey) ++safe;
+        else if (k[e] != kNoKey && (k[e] & mask) == thr)
+          atomicAdd(hist + ((k[e] >> shift) & dmask), 1u);
+      }
+    });
+    // the protected keys fill the top bin of pass 0 alone, and a threshold there ends the search
+    if (pass == 0) {
+      safe = __reduce_add_sync(kFullMask, safe);
+      if (lane == 0 && safe) atomicAdd(hist + dmask, safe);
     }
-    cluster.sync();
+    if (C == 1) __syncthreads();
+    else cluster.sync();
     // bins from the top: thread t owns the 4 bins below kBins - 4 t
     const int bin0 = kBins - 4 - 4 * tid;
-    uint4 sum = make_uint4(0u, 0u, 0u, 0u);
-    for (int r = 0; r < C; ++r) {
-      const uint4 v =
-          *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, r) + bin0);
-      sum.x += v.x;
-      sum.y += v.y;
-      sum.z += v.z;
-      sum.w += v.w;
-    }
-    const uint32_t mine = sum.x + sum.y + sum.z + sum.w;
-    uint32_t inc = mine;
+    uint32_t c[4] = {0u, 0u, 0u, 0u};
+    if (C == 1) {
+      const uint4 v = *reinterpret_cast<const uint4*>(hist + bin0);
+      c[0] = v.x; c[1] = v.y; c[2] = v.z; c[3] = v.w;
+    } else {
+      uint4 v[kMaxCluster];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(kFullMask, inc, o);
-      if (lane >= o) inc += up;
+      for (int r = 0; r < kMaxCluster; ++r)
+        v[r] = r < C ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, r) + bin0)
+                     : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        c[0] += v[r].x; c[1] += v[r].y; c[2] += v[r].z; c[3] += v[r].w;
+      }
     }
+    const uint32_t mine = c[0] + c[1] + c[2] + c[3];
+    const uint32_t inc = warp_inclusive(mine, lane);
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    uint32_t before = inc - mine;
-    for (int w = 0; w < warp; ++w) before += s_scan[w];
-    // the thread in whose bins the count reaches `left` (exactly one: the row has more keys)
-    if (before < left && before + mine >= left) {
-      const uint32_t c[4] = {sum.w, sum.z, sum.y, sum.x};
+    const uint32_t before = below_this_warp(s_scan, warp, lane) + inc - mine;
+    // the thread in whose bins the count reaches `need` (exactly one: the row has more keys)
+    if (before < need && before + mine >= need) {
       uint32_t above = before;
-      int e = 0;
-      while (above + c[e] < left) above += c[e++];
-      s_digit = uint32_t(bin0 + 3 - e);
-      s_left = left - above;
+#pragma unroll
+      for (int e = 3; e >= 0; --e) {
+        if (above < need && above + c[e] >= need) {
+          s_digit = uint32_t(bin0 + e);
+          s_left = need - above;
+          s_bin = c[e];
+        }
+        above += c[e];
+      }
     }
     __syncthreads();
-    prefix |= s_digit << shift;
+    thr |= s_digit << shift;
     mask |= dmask << shift;
-    left = s_left;
+    need = s_left;
+    // the same in every CTA of the cluster: the whole bin is kept, or it is the protected keys'
+    if (s_bin == need || (pass == 0 && s_digit == dmask)) break;
   }
-  const uint32_t thr = prefix, need = left;
 
   // ---- keys above and at the threshold before each warp's slots
   uint32_t gt = 0u, eq = 0u;
-  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t k = i < w_hi ? key_at(i) : 0u;
-    gt += __popc(__ballot_sync(kFullMask, i < w_hi && k > thr));
-    eq += __popc(__ballot_sync(kFullMask, i < w_hi && k == thr));
-  }
+  each_tile([&](int, const uint32_t (&k)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      gt += (k[e] & mask) > thr ? 1u : 0u;
+      eq += (k[e] & mask) == thr && k[e] != kNoKey ? 1u : 0u;
+    }
+  });
+  gt = __reduce_add_sync(kFullMask, gt);
+  eq = __reduce_add_sync(kFullMask, eq);
   if (lane == 0) {
     s_gt[warp] = gt;
     s_eq[warp] = eq;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t g = 0u, q = 0u;
-    for (int w = 0; w < kSelWarps; ++w) {
-      g += s_gt[w];
-      q += s_eq[w];
+  uint32_t gt_before = below_this_warp(s_gt, warp, lane);
+  uint32_t eq_before = below_this_warp(s_eq, warp, lane);
+  if (C > 1) {
+    if (tid == kSelThreads - 1) {
+      s_tot[0] = gt_before + gt;
+      s_tot[1] = eq_before + eq;
     }
-    s_tot[0] = g;
-    s_tot[1] = q;
-  }
-  cluster.sync();
-  uint32_t gt_before = 0u, eq_before = 0u;
-  for (int r = 0; r < rank; ++r) {
-    const uint32_t* t = cluster.map_shared_rank(s_tot, r);
-    gt_before += t[0];
-    eq_before += t[1];
-  }
-  cluster.sync();                            // no CTA ends while another reads its totals
-  for (int w = 0; w < warp; ++w) {
-    gt_before += s_gt[w];
-    eq_before += s_eq[w];
+    cluster.sync();
+    gt = eq = 0u;
+    if (lane < rank) {                       // rank < kMaxCluster lanes
+      const uint32_t* t = cluster.map_shared_rank(s_tot, lane);
+      gt = t[0];
+      eq = t[1];
+    }
+    gt_before += __reduce_add_sync(kFullMask, gt);
+    eq_before += __reduce_add_sync(kFullMask, eq);
+    cluster.sync();                          // no CTA ends while another reads its totals
   }
 
   // ---- the moves: the i-th hole from the front takes the i-th mover from the back
-  const unsigned lower = (1u << lane) - 1u;
-  for (int i0 = w_lo; i0 < w_hi; i0 += 32) {
-    const int i = i0 + lane;
-    const bool in = i < w_hi;
-    const uint32_t k = in ? key_at(i) : 0u;
-    const unsigned g = __ballot_sync(kFullMask, in && k > thr);
-    const unsigned q = __ballot_sync(kFullMask, in && k == thr);
-    const uint32_t eq_at = eq_before + __popc(q & lower);
-    const int kept_before = int(gt_before + __popc(g & lower) + min(eq_at, need));
-    const bool kept = k > thr || (k == thr && eq_at < need);
-    if (in) {
-      if (i < p.budget && !kept) dst[i - kept_before] = i;
-      if (i >= p.budget && kept) src[p.budget - 1 - kept_before] = i;
-      if (i == p.budget - 1) p.counts[row] = p.budget - kept_before - (kept ? 1 : 0);
+  each_tile([&](int i, const uint32_t (&k)[4]) {
+    uint32_t cnt = 0u;                       // above: low half, at the threshold: high half
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cnt += (k[e] & mask) > thr ? 1u : 0u;
+      cnt += (k[e] & mask) == thr && k[e] != kNoKey ? 0x10000u : 0u;
     }
-    gt_before += __popc(g);
-    eq_before += __popc(q);
-  }
+    const uint32_t inc = warp_inclusive(cnt, lane);
+    uint32_t g = gt_before + ((inc - cnt) & 0xffffu), q = eq_before + ((inc - cnt) >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (k[e] == kNoKey) break;
+      const bool is_gt = (k[e] & mask) > thr, is_eq = (k[e] & mask) == thr;
+      const int kept_before = int(g + min(q, need));
+      const bool kept = is_gt || (is_eq && q < need);
+      const int at = i + e;
+      if (at < p.budget && !kept) dst[at - kept_before] = at;
+      if (at >= p.budget && kept) src[p.budget - 1 - kept_before] = at;
+      if (at == p.budget - 1) p.counts[row] = p.budget - kept_before - (kept ? 1 : 0);
+      g += is_gt ? 1u : 0u;
+      q += is_eq ? 1u : 0u;
+    }
+    const uint32_t all = __shfl_sync(kFullMask, inc, 31);
+    gt_before += all & 0xffffu;
+    eq_before += all >> 16;
+  });
 }
 
 // ------------------------------------------------------------------------------ compaction
 //
-// One warp moves kRows rows: all their 16-byte loads are issued before the first store.
+// A warp takes up to 32 moves: each lane looks up one move's pages, so the chain of list, table
+// and rows is paid once for all of them. Then kInFlight 16-byte loads a lane are issued before
+// the first store; rows of at most 16 or 8 chunks share a warp's load.
 
 constexpr int kMoveThreads = 256;
-constexpr int kRows = 4;
+constexpr int kMoveWarps = kMoveThreads / 32;
+constexpr int kInFlight = 8;
 
 struct CacheView {
   uint8_t* base;
@@ -271,80 +327,85 @@ struct CompactParams {
   int32_t* positions;       // nullable
   int64_t pos_sb, pos_sh;
   int slots;                // slots that a row of scores / positions has
+  int lanes;                // lanes that copy a row: 8, 16 or 32
+  int per_warp;             // moves of a warp: kInFlight rows at a time, or 32
   unsigned* status;         // nullable
 };
 
 __global__ void __launch_bounds__(kMoveThreads)
 compact_kernel(const CompactParams p) {
+  __shared__ int4 s_move[kMoveWarps][32];    // page and slot in it, from and to
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = blockIdx.y, b = blockIdx.z;
-  const int i0 = (int(blockIdx.x) * (kMoveThreads / 32) + warp) * kRows;
+  const int i0 = (int(blockIdx.x) * kMoveWarps + warp) * p.per_warp;
   pdl_wait();
   pdl_launch_dependents();
   const int64_t row = int64_t(b) * p.kv_heads + h;
-  const int count = min(p.counts[row], p.moves);
-  if (i0 >= count) return;
+  const int count = min(min(p.counts[row], p.moves) - i0, p.per_warp);
+  if (count <= 0) return;
   const int64_t cap = min(int64_t(p.max_blocks) << p.bs_shift, int64_t(p.slots));
   const int32_t* bt = p.block_table + int64_t(b) * p.bt_sb;
-  int from[kRows], to[kRows];
-  int64_t pf[kRows], pt[kRows];
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const bool in = i0 + u < count;
-    from[u] = in ? p.src[row * p.moves + i0 + u] : -1;
-    to[u] = in ? p.dst[row * p.moves + i0 + u] : -1;
-  }
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    bool ok = from[u] >= 0 && to[u] >= 0;
-    if (ok && (from[u] >= cap || to[u] >= cap)) {
-      if (lane == 0) flag_device_error(p.status, BPT_DEV_SEQ_TOO_LONG);
-      ok = false;
-    }
-    pf[u] = ok ? bt[from[u] >> p.bs_shift] : -1;
-    pt[u] = ok ? bt[to[u] >> p.bs_shift] : -1;
-    if (ok && (pf[u] < 0 || pf[u] >= p.num_blocks || pt[u] < 0 || pt[u] >= p.num_blocks)) {
-      if (lane == 0) flag_device_error(p.status, BPT_DEV_BAD_BLOCK_ID);
-      ok = false;
-    }
-    if (!ok) pf[u] = -1;
-  }
   const int bmask = p.block_size - 1;
-  const int kc = p.k.row_bytes >> 4, total = kc + (p.v.row_bytes >> 4);
-  for (int c = lane; c < total; c += 32) {
-    const CacheView& x = c < kc ? p.k : p.v;
-    uint8_t* col = x.base + int64_t(h) * x.sh + 16 * (c < kc ? c : c - kc);
-    uint4 d[kRows];
-#pragma unroll
-    for (int u = 0; u < kRows; ++u)
-      if (pf[u] >= 0)
-        d[u] = *reinterpret_cast<const uint4*>(col + pf[u] * x.sb + (from[u] & bmask) * x.st);
-#pragma unroll
-    for (int u = 0; u < kRows; ++u)
-      if (pf[u] >= 0)
-        *reinterpret_cast<uint4*>(col + pt[u] * x.sb + (to[u] & bmask) * x.st) = d[u];
-  }
-#pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    if (lane != u || pf[u] < 0) continue;
-    if (p.scores) {
+  if (lane < count) {
+    const int from = p.src[row * p.moves + i0 + lane], to = p.dst[row * p.moves + i0 + lane];
+    bool ok = from >= 0 && to >= 0;
+    if (ok && (from >= cap || to >= cap)) {
+      flag_device_error(p.status, BPT_DEV_SEQ_TOO_LONG);
+      ok = false;
+    }
+    int pf = -1, pt = -1;
+    if (ok) {
+      pf = bt[from >> p.bs_shift];
+      pt = bt[to >> p.bs_shift];
+      if (pf < 0 || pf >= p.num_blocks || pt < 0 || pt >= p.num_blocks) {
+        flag_device_error(p.status, BPT_DEV_BAD_BLOCK_ID);
+        ok = false;
+      }
+    }
+    s_move[warp][lane] = make_int4(ok ? pf : -1, from & bmask, pt, to & bmask);
+    if (ok && p.scores) {
       float* s = p.scores + int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh;
-      s[to[u]] = s[from[u]];
+      s[to] = s[from];
     }
-    if (p.positions) {
+    if (ok && p.positions) {
       int32_t* s = p.positions + int64_t(b) * p.pos_sb + int64_t(h) * p.pos_sh;
-      s[to[u]] = s[from[u]];
+      s[to] = s[from];
     }
   }
+  __syncwarp();
+  const int sub = lane / p.lanes, step = 32 / p.lanes;   // rows that share a load
+  const int kc = p.k.row_bytes >> 4, total = kc + (p.v.row_bytes >> 4);
+  for (int m0 = sub; m0 < count; m0 += kInFlight * step)
+    for (int c = lane % p.lanes; c < total; c += p.lanes) {
+      const bool is_k = c < kc;
+      const int64_t sb = is_k ? p.k.sb : p.v.sb, st = is_k ? p.k.st : p.v.st;
+      uint8_t* col = (is_k ? p.k.base + int64_t(h) * p.k.sh : p.v.base + int64_t(h) * p.v.sh) +
+                     16 * (is_k ? c : c - kc);
+      uint4 d[kInFlight];
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int m = m0 + u * step;
+        if (m >= count) continue;
+        const int4 v = s_move[warp][m];
+        if (v.x >= 0) d[u] = *reinterpret_cast<const uint4*>(col + v.x * sb + v.y * st);
+      }
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u) {
+        const int m = m0 + u * step;
+        if (m >= count) continue;
+        const int4 v = s_move[warp][m];
+        if (v.x >= 0) *reinterpret_cast<uint4*>(col + v.z * sb + v.w * st) = d[u];
+      }
+    }
 }
 
 // ---------------------------------------------------------------------------------- append
 //
-// A token's K rows and V rows are copied 16 bytes a thread, kUnroll tokens of the same column
-// at a time; where an address or stride is not a multiple of 16 bytes, 2 bytes a thread.
+// A token's K rows and V rows are copied 16 bytes a thread, U tokens of the same column at a
+// time; where an address or stride is not a multiple of 16 bytes, 2 bytes a thread.
 
 constexpr int kAppendThreads = 256;
-constexpr int kUnroll = 4;
+constexpr int kPromptTokens = 8;   // U of an append of several tokens
 
 struct AppendParams {
   CacheView k, v;           // paged: block, token, head
@@ -363,7 +424,7 @@ struct AppendParams {
   unsigned* status;         // nullable
 };
 
-template <typename Word>
+template <typename Word, int U>
 __global__ void __launch_bounds__(kAppendThreads)
 append_kernel(const AppendParams p) {
   constexpr int W = int(sizeof(Word));
@@ -371,7 +432,7 @@ append_kernel(const AppendParams p) {
   pdl_launch_dependents();
   const int b = blockIdx.z;
   const int m = min(max(p.new_lens[b], 0), p.max_new);
-  const int t0 = int(blockIdx.x) * kUnroll;
+  const int t0 = int(blockIdx.x) * U;
   if (t0 >= m) return;
   const int start = p.seq_lens[b];
   const int64_t cap = int64_t(p.max_blocks) << p.bs_shift;
@@ -379,9 +440,9 @@ append_kernel(const AppendParams p) {
   const int k_items = p.k_heads * kw, items = k_items + p.v_heads * vw;
   const int c = int(blockIdx.y) * kAppendThreads + int(threadIdx.x);
   const int32_t* bt = p.block_table + int64_t(b) * p.bt_sb;
-  int64_t page[kUnroll];
+  int64_t page[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int64_t slot = int64_t(start) + t0 + u;
     page[u] = -1;
     if (t0 + u >= m) continue;
@@ -405,25 +466,24 @@ append_kernel(const AppendParams p) {
     const int head = e / w, col = (e % w) * W;
     const uint8_t* f = from.base + int64_t(b) * from.sb + int64_t(head) * from.sh + col;
     uint8_t* d = to.base + int64_t(head) * to.sh + col;
-    Word x[kUnroll];
+    Word x[U];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (page[u] >= 0) x[u] = *reinterpret_cast<const Word*>(f + int64_t(t0 + u) * from.st);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (page[u] >= 0)
         *reinterpret_cast<Word*>(d + page[u] * to.sb + ((start + t0 + u) & bmask) * to.st) = x[u];
-    return;
   }
-  const int h = c - items;                   // one thread a head for the token's state
-  if (h >= p.v_heads) return;
+  // the tokens' state: head h is thread h's (there are at least as many columns as heads)
+  if (c >= p.v_heads) return;
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     if (page[u] < 0) continue;
     const int64_t slot = int64_t(start) + t0 + u;
-    if (p.scores) p.scores[int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh + slot] = 0.f;
+    if (p.scores) p.scores[int64_t(b) * p.sc_sb + int64_t(c) * p.sc_sh + slot] = 0.f;
     if (p.positions)
-      p.positions[int64_t(b) * p.pos_sb + int64_t(h) * p.pos_sh + slot] =
+      p.positions[int64_t(b) * p.pos_sb + int64_t(c) * p.pos_sh + slot] =
           p.next_pos[b] + t0 + u;
   }
 }
@@ -460,12 +520,14 @@ bool vec16(const CacheView& v) {
           uintptr_t(v.sh) | uintptr_t(v.row_bytes)) % 16 == 0;
 }
 
-// CTAs per row: enough that the rows fill the SMs, but at least kMinSlots slots a CTA.
+// CTAs per row: enough that the rows fill the SMs, but at least kMinSlots slots a CTA, and more
+// where a slice would not stay in registers.
 int cluster_size(int64_t rows, int slots, int sms) {
   constexpr int kMinSlots = 2048;
   int c = 1;
-  while (c < 8 && ((rows * c * 2 <= sms && slots >= 2 * c * kMinSlots) ||
-                   slots > int64_t(c) * kMaxKeys))
+  while (c < kMaxCluster &&
+         ((rows * c * 2 <= sms && slots >= 2 * c * kMinSlots) ||
+          slots > int64_t(c) * kMaxTiles * kTile * kSelWarps))
     c *= 2;
   return c;
 }
@@ -515,19 +577,18 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   p.moves = bpt_evict_moves(budget, slots);
   p.counts = counts;
   p.new_lens = new_lens;
-  const int per = ((slots + C - 1) / C + kTile - 1) / kTile * kTile;
-  p.key_cap = per < kMaxKeys ? per : kMaxKeys;
   p.vec = ((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(positions)) % 16 ==
            0) &&
           sc_sb % 4 == 0 && sc_sh % 4 == 0 && pos_sb % 4 == 0 && pos_sh % 4 == 0;
-  const size_t smem = size_t(2 * kBins + p.key_cap) * sizeof(uint32_t);
-  if (cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           int((2 * kBins + kMaxKeys) * sizeof(uint32_t))) != cudaSuccess)
-    return BPT_ERR_LAUNCH;
+  // the kernel's own split of the longest row into slices and tiles
+  const int per = cdiv(cdiv(slots, C), kTile) * kTile;
+  const int tiles = cdiv(cdiv(per, kSelWarps), kTile);
+  auto kern = tiles <= 1 ? select_kernel<1> : tiles <= 2 ? select_kernel<2>
+            : tiles <= 4 ? select_kernel<4> : tiles <= 8 ? select_kernel<8>
+            : tiles <= kMaxTiles ? select_kernel<kMaxTiles> : select_kernel<0>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * C));
   cfg.blockDim = dim3(kSelThreads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -538,7 +599,7 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, select_kernel, p) != cudaSuccess) return BPT_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return BPT_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? BPT_OK : BPT_ERR_LAUNCH;
 }
 
@@ -578,8 +639,13 @@ extern "C" int bpt_compact_cache(const bpt_paged_cache* cache, const int32_t* bl
   p.slots = scores || positions ? slots : INT32_MAX;
   p.status = status;
   if (p.kv_heads > kMaxGridYZ || batch > kMaxGridYZ) return BPT_ERR_UNSUPPORTED_SHAPE;
-  constexpr int kPerCta = kMoveThreads / 32 * kRows;
-  const dim3 grid(moves / kPerCta + (moves % kPerCta != 0), p.kv_heads, batch);
+  const int chunks = (p.k.row_bytes + p.v.row_bytes) / 16;
+  p.lanes = chunks > 16 ? 32 : chunks > 8 ? 16 : 8;
+  // few moves: spread them over warps; many: pay the lookups once for 32
+  const int at_once = kInFlight * (32 / p.lanes);
+  p.per_warp = moves > 64 || at_once > 32 ? 32 : at_once;
+  const int per_cta = kMoveWarps * p.per_warp;
+  const dim3 grid(moves / per_cta + (moves % per_cta != 0), p.kv_heads, batch);
   if (launch_dependent(compact_kernel, grid, dim3(kMoveThreads), 0,
                        static_cast<cudaStream_t>(stream), p) != cudaSuccess)
     return BPT_ERR_LAUNCH;
@@ -628,15 +694,16 @@ extern "C" int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new
   const bool vec = vec16(p.k) && vec16(p.v) && vec16(p.kn) && vec16(p.vn);
   const int word = vec ? 16 : 2;
   const int64_t items = int64_t(p.k_heads) * (p.k.row_bytes / word) +
-                        int64_t(p.v_heads) * (p.v.row_bytes / word) + p.v_heads;
+                        int64_t(p.v_heads) * (p.v.row_bytes / word);
   const int64_t blocks = (items + kAppendThreads - 1) / kAppendThreads;
   if (blocks > kMaxGridYZ || batch > kMaxGridYZ) return BPT_ERR_UNSUPPORTED_SHAPE;
-  const int groups = max_new / kUnroll + (max_new % kUnroll != 0);
-  const dim3 grid(groups, unsigned(blocks), batch);
+  const int U = max_new == 1 ? 1 : kPromptTokens;
+  const dim3 grid(max_new / U + (max_new % U != 0), unsigned(blocks), batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e =
-      vec ? launch_dependent(append_kernel<uint4>, grid, dim3(kAppendThreads), 0, st, p)
-          : launch_dependent(append_kernel<uint16_t>, grid, dim3(kAppendThreads), 0, st, p);
+  auto kern = vec ? (U == 1 ? append_kernel<uint4, 1> : append_kernel<uint4, kPromptTokens>)
+                  : (U == 1 ? append_kernel<uint16_t, 1>
+                            : append_kernel<uint16_t, kPromptTokens>);
+  const cudaError_t e = launch_dependent(kern, grid, dim3(kAppendThreads), 0, st, p);
   if (e != cudaSuccess) return BPT_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? BPT_OK : BPT_ERR_LAUNCH;
 }
