@@ -33,9 +33,10 @@ namespace {
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kGroups = kBins / 128;         // a lane's 4 bins times a warp
 constexpr int kTile = 128;                   // slots that a warp takes at a time, 4 a lane
 constexpr int kMaxTiles = 16;                // tiles of a warp that stay in registers
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;                // above 8: not portable, B200 has them
 constexpr uint32_t kProtectedKey = 0xffffffffu;
 constexpr uint32_t kNoKey = 0u;              // past the end; a score's key is at least 1
 
@@ -69,24 +70,26 @@ __device__ __forceinline__ uint32_t warp_inclusive(uint32_t x, int lane) {
   return x;
 }
 
-// Sum of v over the warps below this one: every lane reads one warp's v.
-__device__ __forceinline__ uint32_t below_this_warp(const uint32_t* v, int warp, int lane) {
-  uint32_t x = lane < warp ? v[lane] : 0u;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o);
-  return x;
+// Sum of v[0 .. i), i <= 32.
+__device__ __forceinline__ uint32_t sum_below(const uint32_t* v, int i, int lane) {
+  return __reduce_add_sync(kFullMask, lane < i ? v[lane] : 0u);
 }
 
 template <int TILES>
-__global__ void __launch_bounds__(kSelThreads)
+__global__ void __launch_bounds__(kSelThreads, TILES <= 4 ? 2 : 1)
 select_kernel(const SelectParams p) {
   static_assert(kSelWarps <= 32, "one lane per warp in the block-wide sums");
-  static_assert(kBins == 4 * kSelThreads, "4 bins a thread");
-  __shared__ __align__(16) uint32_t s_hist[2][kBins];
-  __shared__ uint32_t s_scan[kSelWarps];
+  static_assert(kBins == 4 * kSelThreads && kGroups == kSelWarps, "4 bins a thread");
+  static_assert(kMaxCluster <= kSelWarps, "one warp per CTA of the cluster");
+  // a histogram and, past it, one bin that nobody reads for the slots past the end
+  __shared__ __align__(16) uint32_t s_hist[2][kBins + 4];
+  __shared__ uint32_t s_group[2][kGroups];   // sums of 128 bins, from the top
+  // C > 1: the CTAs' group sums, and their bins of the group that is searched
+  __shared__ uint32_t s_groups[kMaxCluster][kGroups];
+  __shared__ __align__(16) uint4 s_bins[kMaxCluster][32];
+  __shared__ uint32_t s_rank_gt[kMaxCluster], s_rank_eq[kMaxCluster];
   __shared__ uint32_t s_digit, s_left, s_bin;
   __shared__ uint32_t s_gt[kSelWarps], s_eq[kSelWarps];
-  __shared__ uint32_t s_tot[2];              // this CTA's keys above and at the threshold
 
   cg::cluster_group cluster = cg::this_cluster();
   const int C = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -165,6 +168,7 @@ select_kernel(const SelectParams p) {
   // ---- the threshold: keys whose masked bits are above thr are kept, of those equal to it the
   // first `need`
   uint32_t thr = 0u, mask = 0u, need = uint32_t(p.budget);
+  uint32_t rank_gt = 0u, rank_eq = 0u;       // warp r: CTA r's keys above and at thr
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
@@ -175,72 +179,124 @@ select_kernel(const SelectParams p) {
       *reinterpret_cast<uint4*>(hist + 4 * tid) = make_uint4(0u, 0u, 0u, 0u);
       __syncthreads();
     }
-    uint32_t safe = 0u;
-    each_tile([&](int, const uint32_t (&k)[4]) {
+    if (pass == 0) {
+      // every key counts, without a branch (the protected ones fill the top bin alone)
+      each_tile([&](int, const uint32_t (&k)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          atomicAdd(hist + (k[e] == kNoKey ? uint32_t(kBins) : k[e] >> 21), 1u);
+      });
+    } else {
+      each_tile([&](int, const uint32_t (&k)[4]) {
+        bool in[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) in[e] = (k[e] & mask) == thr && k[e] != kNoKey;
+        if (!__any_sync(kFullMask, in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (in[e]) atomicAdd(hist + ((k[e] >> shift) & dmask), 1u);
+      });
+    }
+    __syncthreads();
+    // bins from the top: thread t owns the 4 bins from kBins - 4 - 4 t on
+    uint4 c = *reinterpret_cast<const uint4*>(hist + kBins - 4 - 4 * tid);
+    uint32_t sum = c.x + c.y + c.z + c.w, before = 0u, group_sum = 0u;
+    int bin0 = kBins - 4 - 4 * tid, group = 0;
+    if (C == 1) {
+      sum = warp_inclusive(sum, lane);
+      if (lane == 31) s_group[0][warp] = sum;
+      __syncthreads();
+      sum += sum_below(s_group[0], warp, lane);
+    } else {
+      // the CTAs' counts are joined in two steps, warp r fetching CTA r's: the groups of 128
+      // bins, then the bins of the group where the count from the top reaches `need`
+      sum = __reduce_add_sync(kFullMask, sum);
+      if (lane == 0) s_group[pass & 1][warp] = sum;
+      cluster.sync();
+      if (warp < C && lane < kGroups) {
+        group_sum = cluster.map_shared_rank(s_group[pass & 1], warp)[lane];
+        s_groups[warp][lane] = group_sum;
+      }
+      __syncthreads();
+      sum = 0u;
+      if (lane < kGroups)
+        for (int r = 0; r < C; ++r) sum += s_groups[r][lane];
+      const uint32_t inc = warp_inclusive(sum, lane);
+      group = __ffs(__ballot_sync(kFullMask, inc >= need)) - 1;   // the row has more keys
+      before = __shfl_sync(kFullMask, inc - sum, group);
+      bin0 = kBins - 128 * group - 4 - 4 * lane;
+      if (warp < C) {
+        c = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, warp) + bin0);
+        s_bins[warp][lane] = c;
+      }
+      __syncthreads();
+    }
+    if (C == 1 || warp == 0) {
+      uint4 all = c;
+      if (C > 1) {
+        for (int r = 1; r < C; ++r) {
+          const uint4 v = s_bins[r][lane];
+          all.x += v.x; all.y += v.y; all.z += v.z; all.w += v.w;
+        }
+        sum = before + warp_inclusive(all.x + all.y + all.z + all.w, lane);
+      }
+      uint32_t above = sum - (all.x + all.y + all.z + all.w);
+      if (above < need && sum >= need) {     // one thread
+        const uint32_t bin[4] = {all.w, all.z, all.y, all.x};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (above < need && above + bin[e] >= need) {
+            s_digit = uint32_t(bin0 + 3 - e);
+            s_left = need - above;
+            s_bin = bin[e];
+          }
+          above += bin[e];
+        }
+      }
+    }
+    __syncthreads();
+    const uint32_t digit = s_digit;
+    if (C > 1 && warp < C) {                 // CTA `warp`'s keys above and at the digit
+      uint32_t up = lane < group ? group_sum : 0u, at = 0u;
+      const uint32_t bin[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (k[e] == kProtectedKey) ++safe;
-        else if (k[e] != kNoKey && (k[e] & mask) == thr)
-          atomicAdd(hist + ((k[e] >> shift) & dmask), 1u);
+        up += uint32_t(bin0 + e) > digit ? bin[e] : 0u;
+        at += uint32_t(bin0 + e) == digit ? bin[e] : 0u;
       }
-    });
-    // the protected keys fill the top bin of pass 0 alone, and a threshold there ends the search
-    if (pass == 0) {
-      safe = __reduce_add_sync(kFullMask, safe);
-      if (lane == 0 && safe) atomicAdd(hist + dmask, safe);
+      rank_gt += __reduce_add_sync(kFullMask, up);
+      rank_eq = __reduce_add_sync(kFullMask, at);
     }
-    if (C == 1) __syncthreads();
-    else cluster.sync();
-    // bins from the top: thread t owns the 4 bins below kBins - 4 t
-    const int bin0 = kBins - 4 - 4 * tid;
-    uint32_t c[4] = {0u, 0u, 0u, 0u};
-    if (C == 1) {
-      const uint4 v = *reinterpret_cast<const uint4*>(hist + bin0);
-      c[0] = v.x; c[1] = v.y; c[2] = v.z; c[3] = v.w;
-    } else {
-      uint4 v[kMaxCluster];
-#pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r)
-        v[r] = r < C ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(hist, r) + bin0)
-                     : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-      for (int r = 0; r < kMaxCluster; ++r) {
-        c[0] += v[r].x; c[1] += v[r].y; c[2] += v[r].z; c[3] += v[r].w;
-      }
-    }
-    const uint32_t mine = c[0] + c[1] + c[2] + c[3];
-    const uint32_t inc = warp_inclusive(mine, lane);
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    const uint32_t before = below_this_warp(s_scan, warp, lane) + inc - mine;
-    // the thread in whose bins the count reaches `need` (exactly one: the row has more keys)
-    if (before < need && before + mine >= need) {
-      uint32_t above = before;
-#pragma unroll
-      for (int e = 3; e >= 0; --e) {
-        if (above < need && above + c[e] >= need) {
-          s_digit = uint32_t(bin0 + e);
-          s_left = need - above;
-          s_bin = c[e];
-        }
-        above += c[e];
-      }
-    }
-    __syncthreads();
-    thr |= s_digit << shift;
+    thr |= digit << shift;
     mask |= dmask << shift;
     need = s_left;
     // the same in every CTA of the cluster: the whole bin is kept, or it is the protected keys'
-    if (s_bin == need || (pass == 0 && s_digit == dmask)) break;
+    if (s_bin == need || (pass == 0 && digit == dmask)) break;
+  }
+  // where the whole bin is kept, its keys count as above: no ties to rank (a bin at 0 holds NaN
+  // scores and shares the value with the slots past the end)
+  if (s_bin == need && thr != 0u) {
+    thr -= 1u;
+    need = 0u;
+    rank_gt += rank_eq;
+  }
+  const bool ties = need > 0u;
+  if (C > 1) {
+    cluster.barrier_arrive();                // waited for at the end: no CTA ends while read
+    if (warp < C && lane == 0) {
+      s_rank_gt[warp] = rank_gt;
+      s_rank_eq[warp] = rank_eq;
+    }
   }
 
   // ---- keys above and at the threshold before each warp's slots
   uint32_t gt = 0u, eq = 0u;
   each_tile([&](int, const uint32_t (&k)[4]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      gt += (k[e] & mask) > thr ? 1u : 0u;
-      eq += (k[e] & mask) == thr && k[e] != kNoKey ? 1u : 0u;
+    for (int e = 0; e < 4; ++e) gt += (k[e] & mask) > thr ? 1u : 0u;
+    if (ties) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) eq += (k[e] & mask) == thr && k[e] != kNoKey ? 1u : 0u;
     }
   });
   gt = __reduce_add_sync(kFullMask, gt);
@@ -250,52 +306,75 @@ select_kernel(const SelectParams p) {
     s_eq[warp] = eq;
   }
   __syncthreads();
-  uint32_t gt_before = below_this_warp(s_gt, warp, lane);
-  uint32_t eq_before = below_this_warp(s_eq, warp, lane);
+  uint32_t gt_before = sum_below(s_gt, warp, lane);
+  uint32_t eq_before = sum_below(s_eq, warp, lane);
   if (C > 1) {
-    if (tid == kSelThreads - 1) {
-      s_tot[0] = gt_before + gt;
-      s_tot[1] = eq_before + eq;
-    }
-    cluster.sync();
-    gt = eq = 0u;
-    if (lane < rank) {                       // rank < kMaxCluster lanes
-      const uint32_t* t = cluster.map_shared_rank(s_tot, lane);
-      gt = t[0];
-      eq = t[1];
-    }
-    gt_before += __reduce_add_sync(kFullMask, gt);
-    eq_before += __reduce_add_sync(kFullMask, eq);
-    cluster.sync();                          // no CTA ends while another reads its totals
+    gt_before += sum_below(s_rank_gt, rank, lane);
+    eq_before += sum_below(s_rank_eq, rank, lane);
   }
 
   // ---- the moves: the i-th hole from the front takes the i-th mover from the back
+  const unsigned lower = (1u << lane) - 1u;
   each_tile([&](int i, const uint32_t (&k)[4]) {
-    uint32_t cnt = 0u;                       // above: low half, at the threshold: high half
+    bool kept[4];
+    int g = 0;                               // kept slots before this lane's
+    uint32_t here = 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      cnt += (k[e] & mask) > thr ? 1u : 0u;
-      cnt += (k[e] & mask) == thr && k[e] != kNoKey ? 0x10000u : 0u;
+      kept[e] = (k[e] & mask) > thr;
+      const unsigned m = __ballot_sync(kFullMask, kept[e]);
+      g += __popc(m & lower);
+      here += __popc(m);
     }
-    const uint32_t inc = warp_inclusive(cnt, lane);
-    uint32_t g = gt_before + ((inc - cnt) & 0xffffu), q = eq_before + ((inc - cnt) >> 16);
+    g += int(gt_before + min(eq_before, need));
+    gt_before += here;
+    if (ties) {
+      bool is_eq[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (k[e] == kNoKey) break;
-      const bool is_gt = (k[e] & mask) > thr, is_eq = (k[e] & mask) == thr;
-      const int kept_before = int(g + min(q, need));
-      const bool kept = is_gt || (is_eq && q < need);
-      const int at = i + e;
-      if (at < p.budget && !kept) dst[at - kept_before] = at;
-      if (at >= p.budget && kept) src[p.budget - 1 - kept_before] = at;
-      if (at == p.budget - 1) p.counts[row] = p.budget - kept_before - (kept ? 1 : 0);
-      g += is_gt ? 1u : 0u;
-      q += is_eq ? 1u : 0u;
+      for (int e = 0; e < 4; ++e) is_eq[e] = (k[e] & mask) == thr && k[e] != kNoKey;
+      if (__any_sync(kFullMask, is_eq[0] || is_eq[1] || is_eq[2] || is_eq[3])) {
+        uint32_t q = eq_before;
+        here = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned m = __ballot_sync(kFullMask, is_eq[e]);
+          q += __popc(m & lower);
+          here += __popc(m);
+        }
+        g += int(min(q, need)) - int(min(eq_before, need));
+        eq_before += here;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          kept[e] = kept[e] || (is_eq[e] && q < need);
+          q += is_eq[e] ? 1u : 0u;
+        }
+      }
     }
-    const uint32_t all = __shfl_sync(kFullMask, inc, 31);
-    gt_before += all & 0xffffu;
-    eq_before += all >> 16;
+    const int i0 = i - 4 * lane, last = p.budget - 1;
+    if (i0 > last) {                         // movers
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (kept[e]) src[last - g] = i + e;
+        g += kept[e] ? 1 : 0;
+      }
+    } else if (i0 + kTile <= last) {         // holes (k is a slot's: the budget is below n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!kept[e]) dst[i + e - g] = i + e;
+        g += kept[e] ? 1 : 0;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = i + e;
+        if (at <= last && !kept[e]) dst[at - g] = at;
+        if (at > last && kept[e]) src[last - g] = at;
+        if (at == last) p.counts[row] = p.budget - g - (kept[e] ? 1 : 0);
+        g += kept[e] ? 1 : 0;
+      }
+    }
   });
+  if (C > 1) cluster.barrier_wait();
 }
 
 // ------------------------------------------------------------------------------ compaction
@@ -556,8 +635,8 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
       (slots > 0 && (!scores || !positions)))
     return BPT_ERR_INVALID_ARGUMENT;
   const int64_t rows = int64_t(batch) * kv_heads;
+  if (rows > INT32_MAX / kMaxCluster) return BPT_ERR_UNSUPPORTED_SHAPE;
   const int C = cluster_size(rows, slots, device_sm_count());
-  if (rows * C > INT32_MAX) return BPT_ERR_UNSUPPORTED_SHAPE;
   SelectParams p{};
   p.scores = scores;
   p.sc_sb = sc_sb;
@@ -586,6 +665,9 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   auto kern = tiles <= 1 ? select_kernel<1> : tiles <= 2 ? select_kernel<2>
             : tiles <= 4 ? select_kernel<4> : tiles <= 8 ? select_kernel<8>
             : tiles <= kMaxTiles ? select_kernel<kMaxTiles> : select_kernel<0>;
+  if (C > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+                   cudaSuccess)
+    return BPT_ERR_LAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(rows * C));
   cfg.blockDim = dim3(kSelThreads);
