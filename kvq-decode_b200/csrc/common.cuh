@@ -97,6 +97,23 @@ __device__ __forceinline__ uint64_t l2_evict_first_policy() {
   return pol;
 }
 
+__device__ __forceinline__ uint64_t l2_evict_last_policy() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
+__device__ __forceinline__ void store_float2_hint(float* dst, float x, float y, uint64_t policy) {
+  asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(dst), "f"(x), "f"(y),
+               "l"(policy)
+               : "memory");
+}
+
+// Drop a 128-byte line (aligned) whose contents nobody needs: it is not written back to memory.
+__device__ __forceinline__ void discard_line(const void* line) {
+  asm volatile("discard.global.L2 [%0], 128;" ::"l"(line) : "memory");
+}
+
 // 4-D tiled TMA load into this CTA's shared memory, completion signalled on `bar` as
 // transaction bytes. Coordinates are element indices, innermost first. The innermost
 // coordinate passed by the bpt kernels is always 0 (16-byte aligned by construction).

@@ -20,6 +20,8 @@
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "decode_common.h"
 #include "mma_decode.cuh"
@@ -32,6 +34,13 @@ constexpr int kMapWarps = 8;                      // warps that join one map's s
 constexpr int finish_threads(int maps) { return maps * kMapWarps * 32; }
 constexpr int score_tokens_of(int maps) { return 4 * finish_threads(maps); }  // of one CTA
 constexpr int kMaxRows = 8;                       // q rows per kv head
+// Scoring CTAs an SM, each of several rounds: 29 us for 59 MB of logits with a CTA per 1024
+// tokens (B=16, 24-32k tokens, 32 q heads), 20 us with 4 an SM; 8 measured as 4.
+constexpr int kScoreCtas = 4;
+// The logits stay in L2 (evict-last stores). A buffer that would be written back while the next
+// call streams its cache is dropped line by line once read: 306 -> 298 us at 59 MB, 627 -> 620
+// at 114 MB (B=16). At 17 MB dropping costs more than it saves: 89 -> 92 us (B=1, 128k tokens).
+constexpr int64_t kDropBytes = 32 << 20;
 
 // Split CTA shape: 2 warps of 16 tokens each, a 3-stage ring, and as many CTAs an SM as the ring
 // of a width allows (4 at 128 channels, 2 at 256). Width 256 measured with 64-token chunks in 2
@@ -50,6 +59,7 @@ struct FinishParams {
   const float* o_part;  // [B, R, S, D] normalised partial outputs
   const float* logits;  // [B, R, pitch]
   int64_t pitch;
+  int drop_lines;       // drop the logits from L2 once read, instead of writing them back
   const int32_t* seq_lens;
   int64_t cap;
   float* scores;
@@ -64,7 +74,8 @@ struct FinishParams {
   int64_t o_sb, o_sh;
   int kv_heads, group, splits;
   int n_merge;          // CTAs [0, n_merge) join outputs, the others score tokens
-  int out_heads, chunks;
+  int out_heads;
+  int rounds, parts;    // of a scoring CTA, scoring CTAs of a (sequence, kv head)
 };
 
 // (M, 1 / L) of one row over its S splits; every lane gets it. L = 0 (no token) gives 0.
@@ -182,24 +193,35 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
     store16<BF16>(p.out, int64_t(b) * p.o_sb + int64_t(j) * p.o_sh + tid, DIFF ? r * mul : r);
 }
 
-// One CTA's tokens of one (sequence, kv head), 4 a thread.
-template <bool DIFF>
+// The tokens of a CTA, all of one (sequence, kv head): p.rounds times 4 a thread. A round's
+// logits and old scores are asked for while the round before it is worked on, the first ones
+// while the splits' states are joined.
+template <int ROWS, bool DIFF>
 __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, float* s_m,
                                              float* s_inv, float* s_lam) {
+  constexpr int STEP = score_tokens_of(DIFF ? 2 : 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int chunk = id % p.chunks, bh = id / p.chunks;
+  const int part = id % p.parts, bh = id / p.parts;
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
   const int n = int(min(int64_t(max(p.seq_lens[b], 0)), p.cap));
-  const int64_t t0 = int64_t(chunk) * score_tokens_of(DIFF ? 2 : 1);
-  if (t0 >= n) return;                            // uniform over the CTA
+  const int64_t first = int64_t(part) * p.rounds * STEP;
+  if (first >= n) return;                         // uniform over the CTA
+  const int64_t end = min(int64_t(n), first + int64_t(p.rounds) * STEP);
   const int G = p.group;
   const int64_t row0 = int64_t(bh) * G;
-  const int64_t t = t0 + 4 * tid;
-  // the logits are asked for before the splits' states: their latencies overlap
-  float4 x[kMaxRows];
+  const float* logits = p.logits + row0 * p.pitch;
+  float* sc = p.scores + int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh;
+  const bool fades = p.decay != 0.f;
+  auto load = [&](int64_t t, float4 (&x)[ROWS], float4& old) {
+    if (t >= end) return;
 #pragma unroll
-  for (int r = 0; r < kMaxRows; ++r)
-    if (r < G && t < n) x[r] = *reinterpret_cast<const float4*>(p.logits + (row0 + r) * p.pitch + t);
+    for (int r = 0; r < ROWS; ++r)
+      if (r < G) x[r] = *reinterpret_cast<const float4*>(logits + r * p.pitch + t);
+    if (fades && p.score_vec && t + 4 <= n) old = *reinterpret_cast<const float4*>(sc + t);
+  };
+  int64_t t = first + 4 * tid;
+  float4 x[ROWS], old = make_float4(0.f, 0.f, 0.f, 0.f);
+  load(t, x, old);
   if (warp < G) {
     float M, inv;
     row_state(p.m + (row0 + warp) * p.splits, p.l + (row0 + warp) * p.splits, p.splits, lane, M,
@@ -212,41 +234,51 @@ __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, floa
     }
   }
   __syncthreads();
-  if (t >= n) return;
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-  float a[4];
+  for (; t - 4 * lane < end; t += STEP) {         // uniform over the warp
+    float4 y[ROWS], next = make_float4(0.f, 0.f, 0.f, 0.f);
+    load(t + STEP, y, next);
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    float a[4];
 #pragma unroll
-  for (int r = 0; r < kMaxRows; ++r)
-    if (r < G) {
-      const float M = s_m[r], inv = s_inv[r];
-      const float e[4] = {fast_exp2(x[r].x - M) * inv, fast_exp2(x[r].y - M) * inv,
-                          fast_exp2(x[r].z - M) * inv, fast_exp2(x[r].w - M) * inv};
+    for (int r = 0; r < ROWS; ++r)
+      if (r < G) {
+        const float M = s_m[r], inv = s_inv[r];
+        const float e[4] = {fast_exp2(x[r].x - M) * inv, fast_exp2(x[r].y - M) * inv,
+                            fast_exp2(x[r].z - M) * inv, fast_exp2(x[r].w - M) * inv};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (!DIFF) w[i] += e[i];
-        else if ((r & 1) == 0) a[i] = e[i];
-        else w[i] += fabsf(a[i] - s_lam[r] * e[i]);
+        for (int i = 0; i < 4; ++i) {
+          if (!DIFF) w[i] += e[i];
+          else if ((r & 1) == 0) a[i] = e[i];
+          else w[i] += fabsf(a[i] - s_lam[r] * e[i]);
+        }
+      }
+    if (t >= end) {
+      // past the last token of this lane
+    } else if (p.score_vec && t + 4 <= n) {
+      // decay 0 never reads the old scores: its `old` is 0
+      *reinterpret_cast<float4*>(sc + t) =
+          make_float4(fmaf(p.decay, old.x, w[0]), fmaf(p.decay, old.y, w[1]),
+                      fmaf(p.decay, old.z, w[2]), fmaf(p.decay, old.w, w[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t + i < n) sc[t + i] = fades ? fmaf(p.decay, sc[t + i], w[i]) : w[i];
+    }
+    if (p.drop_lines) {                           // every lane of the warp has read its part
+      __syncwarp();
+      if ((lane & 7) == 0 && t < end) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+          if (r < G) discard_line(logits + r * p.pitch + t);
       }
     }
-  float* sc = p.scores + int64_t(b) * p.sc_sb + int64_t(h) * p.sc_sh + t;
-  if (p.score_vec && t + 4 <= n) {
-    float4 o = make_float4(w[0], w[1], w[2], w[3]);
-    if (p.decay != 0.f) {
-      const float4 old = *reinterpret_cast<const float4*>(sc);
-      o.x = fmaf(p.decay, old.x, w[0]);
-      o.y = fmaf(p.decay, old.y, w[1]);
-      o.z = fmaf(p.decay, old.z, w[2]);
-      o.w = fmaf(p.decay, old.w, w[3]);
-    }
-    *reinterpret_cast<float4*>(sc) = o;
-    return;
-  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (t + i < n) sc[i] = p.decay != 0.f ? fmaf(p.decay, sc[i], w[i]) : w[i];
+    for (int r = 0; r < ROWS; ++r) x[r] = y[r];
+    old = next;
+  }
 }
 
-template <int D, bool BF16, bool DIFF>
+template <int D, int ROWS, bool BF16, bool DIFF>
 __global__ void __launch_bounds__(finish_threads(DIFF ? 2 : 1))
 finish_scored_kernel(const FinishParams p) {
   __shared__ __align__(16) float s_o[(DIFF ? 2 : 1) * kMapWarps * D];
@@ -257,7 +289,7 @@ finish_scored_kernel(const FinishParams p) {
   if (int(blockIdx.x) < p.n_merge)
     join_output<D, BF16, DIFF>(p, blockIdx.x, s_o, s_a);
   else
-    score_tokens<DIFF>(p, int(blockIdx.x) - p.n_merge, s_a, s_b, s_c);
+    score_tokens<ROWS, DIFF>(p, int(blockIdx.x) - p.n_merge, s_a, s_b, s_c);
 }
 
 template <int D, bool BF16, bool DIFF>
@@ -265,14 +297,16 @@ int launch_both(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams
                 const FinishParams& f, cudaStream_t st) {
   constexpr int R = resident_ctas(D);
   using Op = mma::OpState<BF16, DIFF>;
-  const int rc = p.group > 4
-                     ? mma::launch<D, kSplitWarps, kStages, R, true, Op>(tk, tv, p, st)
-                     : mma::launch<D, kSplitWarps, kStages, R, false, Op>(tk, tv, p, st);
+  const bool wide = p.group > 4;
+  const int rc = wide ? mma::launch<D, kSplitWarps, kStages, R, true, Op>(tk, tv, p, st)
+                      : mma::launch<D, kSplitWarps, kStages, R, false, Op>(tk, tv, p, st);
   if (rc) return rc;
   const int64_t grid = int64_t(f.n_merge) +
-                       (f.scores ? int64_t(p.batch) * p.kv_heads * f.chunks : 0);
-  return launch_dependent(finish_scored_kernel<D, BF16, DIFF>, dim3(unsigned(grid)),
-                          dim3(finish_threads(DIFF ? 2 : 1)), 0, st, f) == cudaSuccess
+                       (f.scores ? int64_t(p.batch) * p.kv_heads * f.parts : 0);
+  auto finish = wide ? finish_scored_kernel<D, 8, BF16, DIFF>
+                     : finish_scored_kernel<D, 4, BF16, DIFF>;
+  return launch_dependent(finish, dim3(unsigned(grid)), dim3(finish_threads(DIFF ? 2 : 1)), 0, st,
+                          f) == cudaSuccess
              ? BPT_OK
              : BPT_ERR_LAUNCH;
 }
@@ -412,6 +446,8 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   f.o_part = ws.o_part;
   f.logits = ws.logits;
   f.pitch = p.logit_pitch;
+  f.drop_lines = a->scores && !misaligned(ws.logits, 128) &&
+                 int64_t(a->batch) * a->q_heads * f.pitch * 4 >= kDropBytes;
   f.seq_lens = a->seq_lens;
   f.cap = cap;
   f.scores = a->scores;
@@ -433,9 +469,13 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   f.splits = S;
   f.out_heads = a->q_heads / maps;
   f.n_merge = a->batch * f.out_heads;
-  f.chunks = int((cap + score_tokens_of(maps) - 1) / score_tokens_of(maps));
-  if (int64_t(f.n_merge) + int64_t(a->batch) * a->kv_heads * f.chunks > INT32_MAX)
-    return BPT_ERR_UNSUPPORTED_SHAPE;
+  // rounds: one while the CTAs fit the SMs at once, then what keeps them to kScoreCtas an SM
+  const int64_t steps = (cap + score_tokens_of(maps) - 1) / score_tokens_of(maps);
+  const int64_t rows = int64_t(a->batch) * a->kv_heads;
+  const int64_t most = int64_t(kScoreCtas) * device_sm_count();
+  f.rounds = int(std::max<int64_t>(1, std::min<int64_t>(steps, steps * rows / most)));
+  f.parts = int((steps + f.rounds - 1) / f.rounds);
+  if (f.n_merge + rows * f.parts > INT32_MAX) return BPT_ERR_UNSUPPORTED_SHAPE;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = a->dtype == BPT_BF16;
   if (maps == 2)

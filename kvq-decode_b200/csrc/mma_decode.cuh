@@ -349,6 +349,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
   const int colA = 2 * t4, colB = 2 * t4 + 1;
   const int srcA = (G8 ? colA : (colA & 3)) * 4, srcB = (G8 ? colB : (colB & 3)) * 4;
 
+  // the logits are read again by the next kernel, the cache is not: they outlast its stream in L2
+  const uint64_t keep = Op::kState ? l2_evict_last_policy() : 0u;
   for (int c = 0; c < nchunks; ++c) {
     const int stage = c % STAGES;
     const uint32_t par = uint32_t(c / STAGES) & 1u;
@@ -385,8 +387,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       if (p.logits && qvalid && (G8 || g < 4)) {
         float* row = p.logits + (int64_t(b) * p.q_heads + qh0 + qhead) * p.logit_pitch +
                      (u0 + c) * CHUNK + warp * 16 + tk;
-        *reinterpret_cast<float2*>(row) = make_float2(x0, x1);
-        *reinterpret_cast<float2*>(row + 8) = make_float2(x2, x3);
+        store_float2_hint(row, x0, x1, keep);
+        store_float2_hint(row + 8, x2, x3, keep);
       }
     }
     float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
