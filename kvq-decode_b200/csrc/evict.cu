@@ -29,6 +29,13 @@ namespace {
 // again in each pass); histograms and prefix counts are exchanged through distributed shared
 // memory. Ties at the threshold go to the lowest slots, so the result is unique and does not
 // depend on the order in which the histogram's integer atomics arrive.
+//
+// 8 bytes a slot would take 1.3 to 2.2 us in the cases below; what bounds the kernel is a chain
+// of latencies: lengths, keys, and per pass a histogram and its scan (0.9 us in one CTA, 2.5 to 3
+// us across a cluster). Measured: B=32 x 8 heads of 4112 slots 10.0 us (one CTA a row), 8 heads of
+// 128k slots 14.7 us (clusters of 16), B=8 x 8 heads of 16-32k slots 15.3 us (clusters of 2).
+// Keys in shared memory, three passes always and one thread a bin in the exchange: 18.8, 36.7,
+// 30.7 us.
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
@@ -315,42 +322,46 @@ select_kernel(const SelectParams p) {
 
   // ---- the moves: the i-th hole from the front takes the i-th mover from the back
   const unsigned lower = (1u << lane) - 1u;
+  const int last = p.budget - 1;
   each_tile([&](int i, const uint32_t (&k)[4]) {
-    bool kept[4];
-    int g = 0;                               // kept slots before this lane's
-    uint32_t here = 0u;
+    const int i0 = i - 4 * lane;
+    bool kept[4], is_eq[4];
+    unsigned above[4], at_thr[4];
+    uint32_t gts = 0u, eqs = 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       kept[e] = (k[e] & mask) > thr;
-      const unsigned m = __ballot_sync(kFullMask, kept[e]);
-      g += __popc(m & lower);
-      here += __popc(m);
+      above[e] = __ballot_sync(kFullMask, kept[e]);
+      gts += __popc(above[e]);
     }
-    g += int(gt_before + min(eq_before, need));
-    gt_before += here;
     if (ties) {
-      bool is_eq[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) is_eq[e] = (k[e] & mask) == thr && k[e] != kNoKey;
-      if (__any_sync(kFullMask, is_eq[0] || is_eq[1] || is_eq[2] || is_eq[3])) {
-        uint32_t q = eq_before;
-        here = 0u;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const unsigned m = __ballot_sync(kFullMask, is_eq[e]);
-          q += __popc(m & lower);
-          here += __popc(m);
-        }
-        g += int(min(q, need)) - int(min(eq_before, need));
-        eq_before += here;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          kept[e] = kept[e] || (is_eq[e] && q < need);
-          q += is_eq[e] ? 1u : 0u;
-        }
+      for (int e = 0; e < 4; ++e) {
+        is_eq[e] = (k[e] & mask) == thr && k[e] != kNoKey;
+        at_thr[e] = __ballot_sync(kFullMask, is_eq[e]);
+        eqs += __popc(at_thr[e]);
       }
     }
-    const int i0 = i - 4 * lane, last = p.budget - 1;
+    const uint32_t kept_eq = min(eq_before, need), here = gts + min(eq_before + eqs, need) - kept_eq;
+    int g = int(gt_before + kept_eq);        // kept slots before this lane's, from the tile's on
+    uint32_t q = eq_before;
+    gt_before += gts;
+    eq_before += eqs;
+    // all movers and none kept, or all below the budget and none evicted: nothing to write
+    if (i0 > last ? here == 0u : i0 + kTile <= last && here == uint32_t(kTile)) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) g += __popc(above[e] & lower);
+    if (eqs) {
+      const uint32_t q0 = q;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q += __popc(at_thr[e] & lower);
+      g += int(min(q, need)) - int(min(q0, need));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        kept[e] = kept[e] || (is_eq[e] && q < need);
+        q += is_eq[e] ? 1u : 0u;
+      }
+    }
     if (i0 > last) {                         // movers
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -381,11 +392,16 @@ select_kernel(const SelectParams p) {
 //
 // A warp takes up to 32 moves: each lane looks up one move's pages, so the chain of list, table
 // and rows is paid once for all of them. Then kInFlight 16-byte loads a lane are issued before
-// the first store; rows of at most 16 or 8 chunks share a warp's load.
+// the first store; rows of at most 16 or 8 chunks share a warp's load. Bound by memory with rows of
+// 256 bytes at random places: 229 MB (B=8, 16-32k slots to 4096, 8 heads of 128) in 43 us = 5.3
+// TB/s of the 6.5 that a copy of one piece reaches; 4 rows a warp with a lookup each took 82 us,
+// 4 / 16 loads in flight 46.7 / 45.5, 32 moves a warp 43.7, streaming cache hints 44.3. 16 moves
+// a head (B=32) take 3.6 us, five dependent memory latencies and the launch.
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveWarps = kMoveThreads / 32;
 constexpr int kInFlight = 8;
+constexpr int kManyMoves = 16;   // moves of a warp when there are many
 
 struct CacheView {
   uint8_t* base;
@@ -407,7 +423,7 @@ struct CompactParams {
   int64_t pos_sb, pos_sh;
   int slots;                // slots that a row of scores / positions has
   int lanes;                // lanes that copy a row: 8, 16 or 32
-  int per_warp;             // moves of a warp: kInFlight rows at a time, or 32
+  int per_warp;             // moves of a warp, at most 32
   unsigned* status;         // nullable
 };
 
@@ -481,10 +497,13 @@ compact_kernel(const CompactParams p) {
 // ---------------------------------------------------------------------------------- append
 //
 // A token's K rows and V rows are copied 16 bytes a thread, U tokens of the same column at a
-// time; where an address or stride is not a multiple of 16 bytes, 2 bytes a thread.
+// time, the new rows asked for before the page table; where an address or stride is not a
+// multiple of 16 bytes, 2 bytes a thread. Bound by memory: 101 MB (B=8, 1-2k tokens of 8 heads
+// of 128) in 18.3 us = 5.5 TB/s; U = 4 / 8 / 16 took 18.7 / 19.7 / 25.2. One token of each of 64
+// sequences takes 1.9 us, the launch and two memory latencies.
 
 constexpr int kAppendThreads = 256;
-constexpr int kPromptTokens = 8;   // U of an append of several tokens
+constexpr int kPromptTokens = 2;   // U of an append of several tokens
 
 struct AppendParams {
   CacheView k, v;           // paged: block, token, head
@@ -510,16 +529,28 @@ append_kernel(const AppendParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.z;
-  const int m = min(max(p.new_lens[b], 0), p.max_new);
-  const int t0 = int(blockIdx.x) * U;
+  const int new_len = p.new_lens[b], start = p.seq_lens[b];
+  const int m = min(max(new_len, 0), p.max_new), t0 = int(blockIdx.x) * U;
   if (t0 >= m) return;
-  const int start = p.seq_lens[b];
-  const int64_t cap = int64_t(p.max_blocks) << p.bs_shift;
   const int kw = p.k.row_bytes / W, vw = p.v.row_bytes / W;
   const int k_items = p.k_heads * kw, items = k_items + p.v_heads * vw;
   const int c = int(blockIdx.y) * kAppendThreads + int(threadIdx.x);
+  const bool is_k = c < k_items;
+  const int e = is_k ? c : c - k_items, w = is_k ? kw : vw;
+  const int head = e / w, col = (e % w) * W;
+  // the new rows do not wait for the table
+  Word x[U];
+  if (c < items) {
+    const CacheView& from = is_k ? p.kn : p.vn;
+    const uint8_t* f = from.base + int64_t(b) * from.sb + int64_t(t0) * from.st +
+                       int64_t(head) * from.sh + col;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t0 + u < m) x[u] = *reinterpret_cast<const Word*>(f + int64_t(u) * from.st);
+  }
+  const int64_t cap = int64_t(p.max_blocks) << p.bs_shift;
   const int32_t* bt = p.block_table + int64_t(b) * p.bt_sb;
-  int64_t page[U];
+  int page[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t slot = int64_t(start) + t0 + u;
@@ -538,17 +569,8 @@ append_kernel(const AppendParams p) {
   }
   const int bmask = p.block_size - 1;
   if (c < items) {
-    const bool is_k = c < k_items;
     const CacheView& to = is_k ? p.k : p.v;
-    const CacheView& from = is_k ? p.kn : p.vn;
-    const int e = is_k ? c : c - k_items, w = is_k ? kw : vw;
-    const int head = e / w, col = (e % w) * W;
-    const uint8_t* f = from.base + int64_t(b) * from.sb + int64_t(head) * from.sh + col;
     uint8_t* d = to.base + int64_t(head) * to.sh + col;
-    Word x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (page[u] >= 0) x[u] = *reinterpret_cast<const Word*>(f + int64_t(t0 + u) * from.st);
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (page[u] >= 0)
@@ -723,9 +745,9 @@ extern "C" int bpt_compact_cache(const bpt_paged_cache* cache, const int32_t* bl
   if (p.kv_heads > kMaxGridYZ || batch > kMaxGridYZ) return BPT_ERR_UNSUPPORTED_SHAPE;
   const int chunks = (p.k.row_bytes + p.v.row_bytes) / 16;
   p.lanes = chunks > 16 ? 32 : chunks > 8 ? 16 : 8;
-  // few moves: spread them over warps; many: pay the lookups once for 32
+  // few moves: spread them over warps; many: pay the lookups once for two loads' worth
   const int at_once = kInFlight * (32 / p.lanes);
-  p.per_warp = moves > 64 || at_once > 32 ? 32 : at_once;
+  p.per_warp = moves > 64 && at_once < kManyMoves ? kManyMoves : at_once;
   const int per_cta = kMoveWarps * p.per_warp;
   const dim3 grid(moves / per_cta + (moves % per_cta != 0), p.kv_heads, batch);
   if (launch_dependent(compact_kernel, grid, dim3(kMoveThreads), 0,

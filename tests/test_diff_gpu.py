@@ -72,7 +72,7 @@ def test_diff_lam_zero_is_the_first_map():
 
 
 def test_diff_equal_maps_cancel():
-    """lam 1 and two equal maps: every weight is 0, so out is 0 and the norm does not divide by 0."""
+    """lam 1 and two equal maps: every weight is 0, so out is 0 and the norm divides by no 0."""
     c = attend_case(4, [70, 3], 4, 2, 64, 16, FP16, maps=2)
     c["q"][:, 1::2] = c["q"][:, ::2]
     c["k"][:, :, 1::2] = c["k"][:, :, ::2]

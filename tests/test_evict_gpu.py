@@ -321,8 +321,8 @@ def test_select_long_rows(T, B, H, kind):
 
 
 def test_select_views_reuse_and_too_many_protected():
-    """Unaligned rows of wider buffers; moves reused; positions that protect more than the budget (as a
-    caller's mistake could) still keep exactly the budget."""
+    """Unaligned rows of wider buffers; moves reused; positions that protect more than the budget
+    (as a caller's mistake could) still keep exactly the budget."""
     from bpt import evict
     from oracle import evict as ox
     T, budget = 700, 200
@@ -341,6 +341,35 @@ def test_select_views_reuse_and_too_many_protected():
             assert np.array_equal(got.cpu().numpy(), w)
         m.src.fill_(5)
         m.dst.fill_(5)
+
+
+def test_select_of_a_cluster_in_a_graph_and_on_two_streams():
+    """Long rows (a cluster each): captured and replayed with new scores, and two calls at once."""
+    from bpt import evict
+    T, budget = 60000, 5000
+    a = [x.cuda() for x in select_case(3, 1, 2, T, [T], 64, "weights")]
+    b = [x.cuda() for x in select_case(4, 1, 2, T, [T - 7], 64, "weights")]
+    want = [[t.clone() for t in evict.select_evictions(s, p, n, n, budget, recent=64)]
+            for s, p, n in (a, b)]
+    live = [x.clone() for x in a]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        m = evict.select_evictions(*live, live[2], budget, recent=64)
+    for case, w in ((a, want[0]), (b, want[1]), (a, want[0])):
+        for x, y in zip(live, case):
+            x.copy_(y)
+        g.replay()
+        assert all(torch.equal(x, y) for x, y in zip(m, w))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for st, (s, p, n) in zip(streams, (a, b)):
+            with torch.cuda.stream(st):
+                got.append(evict.select_evictions(s, p, n, n, budget, recent=64))
+        torch.cuda.synchronize()
+        for x, w in zip(got, want):
+            assert all(torch.equal(i, j) for i, j in zip(x, w))
 
 
 # ---------------------------------------------------------------------------- compaction
@@ -376,6 +405,26 @@ def test_evict_and_compact(dtype, H, DK, DV, bs):
     m = evict.EvictionMoves(*(torch.from_numpy(x).cuda() for x in (src, dst, counts, new)))
     evict.compact_cache(gk, gv, bt.cuda(), m)
     assert np.array_equal(f64(gk), want[0]) and np.array_equal(f64(gv), want[1])
+
+
+def test_append_and_compact_far_pages():
+    """Pages past 2^31 elements of a cache (4.5 GB each) are written where the table says."""
+    from bpt import evict
+    bs, H, D = 256, 8, 128
+    nb = (1 << 31) // (bs * H * D) + 16
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = (torch.empty(nb, bs, H, D, dtype=FP16, device="cuda") for _ in "kv")
+    far = i32(nb - 1, nb - 5).view(1, 2)
+    kn, vn = (torch.randn(1, 300, H, D, device="cuda").half() for _ in "kv")
+    evict.append_tokens(k, v, kn, vn, i32(300), i32(0), far)
+    src = torch.arange(299, 289, -1, device="cuda").int().expand(1, H, 10).contiguous()
+    dst = torch.arange(10, device="cuda").int().expand(1, H, 10).contiguous()
+    m = evict.EvictionMoves(src, dst, torch.full((1, H), 10, device="cuda").int(), i32(290))
+    evict.compact_cache(k, v, far, m)
+    for x, new in ((k, kn), (v, vn)):
+        assert torch.equal(x[nb - 5, :44], new[0, 256:])
+        assert torch.equal(x[nb - 1, 10:], new[0, 10:256])
+        assert torch.equal(x[nb - 1, :10], new[0, 290:300].flip(0))
 
 
 def test_compact_checked_mode(monkeypatch):
@@ -468,8 +517,8 @@ def test_serving_loop(maps):
 
 
 def test_step_captured_in_one_graph():
-    """append, decode and eviction of a fixed batch captured once and replayed: lengths and positions
-    advance on the device."""
+    """append, decode and eviction of a fixed batch captured once and replayed: lengths and
+    positions advance on the device."""
     from bpt import evict
     torch.manual_seed(5)
     B, H, D, bs, mb, budget = 3, 2, 64, 16, 6, 64
