@@ -31,10 +31,11 @@ namespace {
 // depend on the order in which the histogram's integer atomics arrive.
 //
 // 8 bytes a slot would take 1.3 to 2.2 us in the cases below; what bounds the kernel is a chain
-// of latencies: lengths, keys, and per pass a histogram and its scan (0.9 us in one CTA, 2.5 to 3
-// us across a cluster). Measured: B=32 x 8 heads of 4112 slots 10.0 us (one CTA a row), 8 heads of
-// 128k slots 14.7 us (clusters of 16), B=8 x 8 heads of 16-32k slots 15.3 us (clusters of 2).
-// Keys in shared memory, three passes always and one thread a bin in the exchange: 18.8, 36.7,
+// of latencies: lengths, keys (1.7 us together), and per pass a histogram and its scan (1 us in
+// one CTA, 2.5 to 3 us across a cluster). Measured: B=32 x 8 heads of 4112 slots 7.0 us (one CTA
+// a row; 10.0 when the zero scores shared a bin and took all three passes), 8 heads of 128k slots
+// 14.7 us (clusters of 16; 15.4 with 8), B=8 x 8 heads of 16-32k slots 14.7 us (clusters of 4; 16.4
+// with 2). The simple form, keys in shared memory and three passes always, took 18.8, 36.7 and
 // 30.7 us.
 
 constexpr int kSelThreads = 512;
@@ -45,6 +46,8 @@ constexpr int kTile = 128;                   // slots that a warp takes at a tim
 constexpr int kMaxTiles = 16;                // tiles of a warp that stay in registers
 constexpr int kMaxCluster = 16;                // above 8: not portable, B200 has them
 constexpr uint32_t kProtectedKey = 0xffffffffu;
+constexpr uint32_t kBinKeys = 1u << 21;      // keys of one bin of the first pass
+constexpr uint32_t kZeroBin = 1024u, kProtectedBin = 2047u;
 constexpr uint32_t kNoKey = 0u;              // past the end; a score's key is at least 1
 
 struct SelectParams {
@@ -62,10 +65,14 @@ struct SelectParams {
   int vec;                                   // rows are 16-byte aligned
 };
 
-// Unsigned key of the same order as the score: NaN lowest, -0 equal to +0.
+// Unsigned key of the same order as the score: NaN lowest, -0 equal to +0. Positive scores are
+// one bin of the first pass higher than their bits, so that 0, the score of new tokens and of
+// weights that underflow, has a bin for itself and a threshold there needs no further pass.
 __device__ __forceinline__ uint32_t score_key(float f) {
   const uint32_t u = __float_as_uint(f + 0.f);
-  return f != f ? 1u : u ^ ((u & 0x80000000u) ? 0xffffffffu : 0x80000000u);
+  if (f != f) return 1u;
+  if (u & 0x80000000u) return ~u;
+  return u + (u ? 0x80000000u + kBinKeys : 0x80000000u);
 }
 
 __device__ __forceinline__ uint32_t warp_inclusive(uint32_t x, int lane) {
@@ -187,7 +194,7 @@ select_kernel(const SelectParams p) {
       __syncthreads();
     }
     if (pass == 0) {
-      // every key counts, without a branch (the protected ones fill the top bin alone)
+      // every key counts, without a branch
       each_tile([&](int, const uint32_t (&k)[4]) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -277,8 +284,8 @@ select_kernel(const SelectParams p) {
     thr |= digit << shift;
     mask |= dmask << shift;
     need = s_left;
-    // the same in every CTA of the cluster: the whole bin is kept, or it is the protected keys'
-    if (s_bin == need || (pass == 0 && digit == dmask)) break;
+    // the same in every CTA of the cluster: the whole bin is kept, or it holds one key only
+    if (s_bin == need || (pass == 0 && (digit == kZeroBin || digit == kProtectedBin))) break;
   }
   // where the whole bin is kept, its keys count as above: no ties to rank (a bin at 0 holds NaN
   // scores and shares the value with the slots past the end)
@@ -621,13 +628,13 @@ bool vec16(const CacheView& v) {
           uintptr_t(v.sh) | uintptr_t(v.row_bytes)) % 16 == 0;
 }
 
-// CTAs per row: enough that the rows fill the SMs, but at least kMinSlots slots a CTA, and more
-// where a slice would not stay in registers.
+// CTAs per row: enough to put two on every SM, but at least kMinSlots slots a CTA, and more where
+// a slice would not stay in registers.
 int cluster_size(int64_t rows, int slots, int sms) {
   constexpr int kMinSlots = 2048;
   int c = 1;
   while (c < kMaxCluster &&
-         ((rows * c * 2 <= sms && slots >= 2 * c * kMinSlots) ||
+         ((rows * c <= sms && slots >= 2 * c * kMinSlots) ||
           slots > int64_t(c) * kMaxTiles * kTile * kSelWarps))
     c *= 2;
   return c;
