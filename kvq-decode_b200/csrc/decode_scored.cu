@@ -30,10 +30,11 @@ namespace bpt {
 namespace {
 
 constexpr float kNegInf = -INFINITY;
-constexpr int kMapWarps = 8;                      // warps that join one map's splits
-constexpr int finish_threads(int maps) { return maps * kMapWarps * 32; }
-constexpr int score_tokens_of(int maps) { return 4 * finish_threads(maps); }  // of one CTA
+constexpr int kFinishWarps = 8;
+constexpr int kFinishThreads = kFinishWarps * 32;
+constexpr int kScoreTokens = 4 * kFinishThreads;  // tokens of a round of a scoring CTA
 constexpr int kMaxRows = 8;                       // q rows per kv head
+static_assert(kMaxRows >= kFinishWarps, "shared rows double as one value a warp");
 // Scoring CTAs an SM, each of several rounds: 29 us for 59 MB of logits with a CTA per 1024
 // tokens (B=16, 24-32k tokens, 32 q heads), 20 us with 4 an SM; 8 measured as 4.
 constexpr int kScoreCtas = 4;
@@ -111,18 +112,20 @@ __device__ __forceinline__ void store16(void* base, int64_t at, float x) {
     static_cast<__half*>(base)[at] = __float2half_rn(x);
 }
 
-// One output row (b, j): sum over its maps and splits of sign * (share of the split) * o. Warps
-// 8 k .. 8 k + 7 join map k; the first U rows of a warp are asked for before the row's
-// state, so that up to 8 U splits cost one memory round trip.
+// One output row (b, j): sum over its maps and splits of sign * (share of the split) * o. The
+// warps are shared out to the maps; the first U rows of a warp are asked for before the row's
+// state, so that 64 splits (32 of 256 channels) cost one memory round trip. 16 warps with DIFF, 8 a
+// map, left one CTA an SM for the scoring: 83.4 us against 81.4 (B=8, 16k tokens, 4 value heads of
+// 256).
 template <int D, bool BF16, bool DIFF>
 __device__ __forceinline__ void join_output(const FinishParams& p, int id, float* s_o,
                                             float* s_red) {
   constexpr int MAPS = DIFF ? 2 : 1;
-  constexpr int WARPS = MAPS * kMapWarps;
+  constexpr int WARPS = kFinishWarps / MAPS;       // of one map
   constexpr int V4 = (D + 127) / 128;             // float4 columns of a lane
-  constexpr int U = V4 == 1 ? 8 : 4;              // rows in flight
+  constexpr int U = MAPS * (V4 == 1 ? 8 : 4);     // rows in flight
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int map = warp / kMapWarps, w0 = warp % kMapWarps;
+  const int map = warp / WARPS, w0 = warp % WARPS;
   const int b = id / p.out_heads, j = id % p.out_heads;
   const int S = p.splits;
   const int64_t row = (int64_t(b) * p.out_heads + j) * MAPS + map;
@@ -133,12 +136,12 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
 #pragma unroll
   for (int v = 0; v < V4; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = 0.f, inv = 0.f;
-  for (int s0 = w0; s0 < S; s0 += kMapWarps * U) {
+  for (int s0 = w0; s0 < S; s0 += WARPS * U) {
     float ms[U], ls[U];
     float4 x[U][V4];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = s0 + kMapWarps * u;
+      const int s = s0 + WARPS * u;
       const bool in = s < S;
       ms[u] = in ? m[s] : 0.f;
       ls[u] = in ? l[s] : 0.f;
@@ -174,7 +177,7 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
   float r = 0.f;
   if (tid < D) {
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) r += s_o[w * D + tid];
+    for (int w = 0; w < kFinishWarps; ++w) r += s_o[w * D + tid];
   }
   float mul = p.out_scale;
   if (DIFF && p.norm_w) {                         // uniform over the CTA
@@ -199,7 +202,7 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
 template <int ROWS, bool DIFF>
 __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, float* s_m,
                                              float* s_inv, float* s_lam) {
-  constexpr int STEP = score_tokens_of(DIFF ? 2 : 1);
+  constexpr int STEP = kScoreTokens;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int part = id % p.parts, bh = id / p.parts;
   const int b = bh / p.kv_heads, h = bh % p.kv_heads;
@@ -279,10 +282,10 @@ __device__ __forceinline__ void score_tokens(const FinishParams& p, int id, floa
 }
 
 template <int D, int ROWS, bool BF16, bool DIFF>
-__global__ void __launch_bounds__(finish_threads(DIFF ? 2 : 1))
+__global__ void __launch_bounds__(kFinishThreads)
 finish_scored_kernel(const FinishParams p) {
-  __shared__ __align__(16) float s_o[(DIFF ? 2 : 1) * kMapWarps * D];
-  __shared__ float s_a[2 * kMapWarps], s_b[kMaxRows], s_c[kMaxRows];
+  __shared__ __align__(16) float s_o[kFinishWarps * D];
+  __shared__ float s_a[kMaxRows], s_b[kMaxRows], s_c[kMaxRows];
   pdl_wait();
   // the next call's split kernel may start launching; it waits for this grid's end
   pdl_launch_dependents();
@@ -305,8 +308,8 @@ int launch_both(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams
                        (f.scores ? int64_t(p.batch) * p.kv_heads * f.parts : 0);
   auto finish = wide ? finish_scored_kernel<D, 8, BF16, DIFF>
                      : finish_scored_kernel<D, 4, BF16, DIFF>;
-  return launch_dependent(finish, dim3(unsigned(grid)), dim3(finish_threads(DIFF ? 2 : 1)), 0, st,
-                          f) == cudaSuccess
+  return launch_dependent(finish, dim3(unsigned(grid)), dim3(kFinishThreads), 0, st, f) ==
+                 cudaSuccess
              ? BPT_OK
              : BPT_ERR_LAUNCH;
 }
@@ -470,7 +473,7 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   f.out_heads = a->q_heads / maps;
   f.n_merge = a->batch * f.out_heads;
   // rounds: one while the CTAs fit the SMs at once, then what keeps them to kScoreCtas an SM
-  const int64_t steps = (cap + score_tokens_of(maps) - 1) / score_tokens_of(maps);
+  const int64_t steps = (cap + kScoreTokens - 1) / kScoreTokens;
   const int64_t rows = int64_t(a->batch) * a->kv_heads;
   const int64_t most = int64_t(kScoreCtas) * device_sm_count();
   f.rounds = int(std::max<int64_t>(1, std::min<int64_t>(steps, steps * rows / most)));
