@@ -346,11 +346,20 @@ ScoredView scored_view(void* ws, int batch, int rows, int width, int splits, int
   return v;
 }
 
+// The shared planner's count, but one chunk a split where that still is one wave (the planner
+// keeps two): B=1, 8 kv heads of 128, 512 / 1024 / 2048 tokens 6.3 / 6.6 / 7.5 us against 7.1 / 7.5 /
+// 8.1 with two.
 int state_splits(int width, int batch, int kv_heads, int block_size, int max_blocks,
                  int num_splits, int sm_count) {
-  const int s = num_splits > 0 ? num_splits
-                               : plan_splits(batch, kv_heads, block_size, max_blocks, sm_count,
-                                             resident_ctas(width), kChunk);
+  const int resident = resident_ctas(width);
+  int s = num_splits;
+  if (s <= 0) {
+    if (sm_count <= 0) sm_count = device_sm_count();
+    const int64_t chunks = (int64_t(max_blocks) * block_size + kChunk - 1) / kChunk;
+    s = chunks * batch * kv_heads <= int64_t(sm_count) * resident
+            ? int(chunks)
+            : plan_splits(batch, kv_heads, block_size, max_blocks, sm_count, resident, kChunk);
+  }
   return clamp_splits(s, block_size, max_blocks, kChunk);
 }
 

@@ -349,7 +349,8 @@ select_kernel(const SelectParams p) {
         eqs += __popc(at_thr[e]);
       }
     }
-    const uint32_t kept_eq = min(eq_before, need), here = gts + min(eq_before + eqs, need) - kept_eq;
+    const uint32_t kept_eq = min(eq_before, need);
+    const uint32_t here = gts + min(eq_before + eqs, need) - kept_eq;
     int g = int(gt_before + kept_eq);        // kept slots before this lane's, from the tile's on
     uint32_t q = eq_before;
     gt_before += gts;

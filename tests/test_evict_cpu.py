@@ -226,6 +226,24 @@ def test_abi_decode_workspace():
     assert lib.bpt_decode_scored(None, None, ctypes.c_size_t(0), None) == _lib.ERR_INVALID_ARGUMENT
 
 
+def test_abi_decode_splits():
+    """One 32-token chunk a split while that is one wave of 4 (width 256: 2) CTAs an SM, else the
+    decode planner's count; requests are clamped to the chunks."""
+    f = _lib.lib().bpt_effective_splits_scored
+    plan = _lib.lib().bpt_plan_splits
+
+    def splits(*x):
+        return f(*[c_i32(i) for i in x])
+    assert splits(128, 1, 1, 8, 16, 64, 0, 148) == 32       # 1024 tokens, 256 CTAs
+    assert splits(64, 2, 1, 8, 16, 64, 0, 148) == 32        # differential, the same width
+    assert splits(128, 1, 1, 8, 16, 256, 0, 148) == plan(1, 8, 16, 256, 148) == 64
+    assert splits(128, 1, 64, 8, 16, 4096, 0, 148) == plan(64, 8, 16, 4096, 148)
+    assert splits(128, 2, 1, 8, 16, 128, 0, 148) == 32      # 512 CTAs of one chunk are 2 waves
+    assert splits(128, 2, 8, 4, 32, 512, 0, 148) == 9       # 2 CTAs an SM: 296 / 32
+    assert splits(128, 1, 2, 8, 16, 4, 7, 148) == 2
+    assert splits(128, 1, 1, 8, 16, 0, 0, 148) == 1
+
+
 def cache_args(**kw):
     c = PagedCache(block_size=16, k_heads=2, v_heads=2, k_dim=64, v_dim=64, num_blocks=4,
                    k=0x100000, v=0x200000)
