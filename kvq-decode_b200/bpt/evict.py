@@ -22,9 +22,15 @@ and, when a sequence has grown past its budget (all layers have their own state)
 
 after which every sequence has at most ``budget`` tokens, in slots 0 .. new_len - 1: the pages
 past them are free. Evicted caches hold their tokens out of order, which attention does not
-notice; keys carry their rotary position from when they were written. Sequences that share
-pages (a common prefix) can be decoded and scored together, but a sequence that is appended to
-or evicted must own its pages alone. ``bpt.diff`` has the differential decode over such a cache.
+notice; keys carry their rotary position from when they were written.
+
+Without a host synchronisation the calls plan for the table's and the rows' width, not for
+the lengths. Where the caller knows that no sequence is longer than n slots, views of that width
+(``block_table[:, :ceil(n / block_size)]``, ``scores[:, :, :n]``) save workspace, splits and CTAs.
+
+Sequences that share pages (a common prefix) can be decoded and scored together, but a sequence
+that is appended to or evicted must own its pages alone. ``bpt.diff`` has the differential decode
+over such a cache.
 """
 import ctypes
 from typing import NamedTuple, Optional

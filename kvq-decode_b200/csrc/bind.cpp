@@ -211,6 +211,7 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
   const int64_t out_heads = Hq / maps;
   if (scores) check_state(*scores, "scores", kF32, B, H, cap, true);
   REQUIRE(std::isfinite(decay) && decay >= 0.0, "decay must be finite and not negative");
+  REQUIRE(!scale || (std::isfinite(*scale) && *scale > 0.0), "scale must be positive and finite");
   if (maps == 2) {
     REQUIRE(lam && lam->scalar_type() == kF32 &&
                 ((lam->dim() == 1 && lam->size(0) == out_heads) ||

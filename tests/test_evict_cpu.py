@@ -86,6 +86,17 @@ def test_scored_refuses_decay(decay):
         scored(tensors(), decay=decay)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf")])
+def test_refuses_scale(scale):
+    """The C ABI takes a scale <= 0 for the default; Python has None for that."""
+    with pytest.raises(BptArgumentError, match="scale"):
+        scored(tensors(), scale=scale)
+    t = tensors(maps=2)
+    with pytest.raises(BptArgumentError, match="scale"):
+        diff.paged_decode_attention_diff(t["q"], t["k"], t["v"], t["bt"], t["sl"],
+                                         torch.zeros(2), scale=scale)
+
+
 def test_scored_needs_scores():
     t = tensors()
     t["scores"] = None

@@ -296,10 +296,11 @@ def plain_select(scores, pos, n, nxt, budget, recent, sinks):
 
 
 @pytest.mark.parametrize("T,B,H", [(131072, 1, 2), (70001, 2, 1), (20000, 3, 5), (450000, 1, 1),
-                                   (120000, 1, 80)])
+                                   (120000, 1, 80), (600001, 1, 1)])
 @pytest.mark.parametrize("kind", ["weights", "same"])
 def test_select_long_rows(T, B, H, kind):
-    """Rows that a cluster shares; the last two are longer than its shared memory holds."""
+    """Rows that a cluster shares: few and many of them, slices of 1 to 16 tiles a warp, and one
+    longer than the registers of the largest cluster hold (read again in each pass)."""
     from bpt import evict
     lens = [T - 13 * b for b in range(B)]
     scores, pos, sl = select_case(T, B, H, T, lens, 1024, kind)
@@ -318,6 +319,26 @@ def test_select_long_rows(T, B, H, kind):
                 assert np.array_equal(src[b, h, :c], movers[::-1])
                 assert np.array_equal(dst[b, h, :c], holes)
                 assert (src[b, h, c:] == -1).all() and (dst[b, h, c:] == -1).all()
+
+
+def test_views_of_short_rows():
+    """A wide table and wide state rows, called through views of the slots in use: the same results
+    as with the whole rows."""
+    from bpt import evict
+    c = attend_case(21, [300, 77], 4, 2, 64, 16, FP16)
+    wide = torch.zeros(2, 4096 // 16, dtype=torch.int32, device="cuda")
+    wide[:, :c["bt"].shape[1]] = c["bt"]
+    scores = torch.zeros(2, 2, 4096, device="cuda")
+    pos = torch.arange(4096, device="cuda").int().expand(2, 2, -1).contiguous()
+    got = []
+    for slots in (4096, 320):
+        s = scores.clone()
+        out = evict.paged_decode_attention_scored(c["q"], c["k"], c["v"], wide[:, :slots // 16],
+                                                  c["sl"], s[:, :, :slots], num_splits=4)
+        m = evict.select_evictions(s[:, :, :slots], pos[:, :, :slots], c["sl"], c["sl"], 100)
+        got.append((out, s, m.src[:, :, :100], m.dst[:, :, :100], m.counts, m.new_lens))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 def test_select_views_reuse_and_too_many_protected():
