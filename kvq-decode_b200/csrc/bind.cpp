@@ -8,6 +8,7 @@
 // the library that bpt._lib loaded.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -247,12 +248,17 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
   const size_t need =
       g_abi.workspace_bytes(int(D), maps, int(B), int(Hq), S, scores ? cap : 0);
   Tensor out = out_arg ? *out_arg : at::empty({B, out_heads, width}, q.options());
-  Tensor ws;
+  // without a workspace: memory of this stream's pool, given back (in stream order) on return
+  void* ws = nullptr;
+  size_t ws_bytes = need;
+  c10::DataPtr own_ws;
   if (workspace_arg && workspace_arg->nbytes() >= need) {
     REQUIRE(workspace_arg->is_contiguous(), "workspace must be contiguous");
-    ws = *workspace_arg;
+    ws = workspace_arg->data_ptr();
+    ws_bytes = workspace_arg->nbytes();
   } else {
-    ws = at::empty({int64_t(need)}, q.options().dtype(at::ScalarType::Byte));
+    own_ws = c10::cuda::CUDACachingAllocator::get()->allocate(need);
+    ws = own_ws.get();
   }
   bpt_scored_decode a = {};
   a.dtype = c.bf16 ? BPT_BF16 : BPT_FP16;
@@ -294,7 +300,7 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
     a.lam_stride[1] = lam->stride(-1);
   }
   a.norm_weight = ptr<float>(norm_weight);
-  check(g_abi.decode(&a, ws.data_ptr(), ws.nbytes(),
+  check(g_abi.decode(&a, ws, ws_bytes,
                      c10::cuda::getCurrentCUDAStream(on.dev.index()).stream()),
         "bpt_decode_scored");
   return out;
