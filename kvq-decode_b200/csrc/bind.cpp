@@ -43,8 +43,12 @@ void bind_to(F& fn, const py::dict& table, const char* name) {
 }
 
 [[noreturn]] void refuse(const std::string& why) {
-  PyErr_SetString(g_argument_error, why.c_str());
+  PyErr_SetString(g_argument_error ? g_argument_error : PyExc_RuntimeError, why.c_str());
   throw py::error_already_set();
+}
+
+void require_init() {
+  if (__builtin_expect(!g_abi.compact, 0)) refuse("bpt/_bind is used through bpt.evict and bpt.diff");
 }
 
 // The message is built only for a call that is refused.
@@ -178,6 +182,7 @@ bpt_paged_cache cache_c(const Tensor& k, const Tensor& v, const Cache& c) {
 
 int64_t scored_workspace_bytes(int maps, const Tensor& q, const Tensor& k_cache,
                                const Tensor& block_table, int num_splits, bool scored) {
+  require_init();
   REQUIRE(q.dim() == 3 && k_cache.dim() == 4 && block_table.dim() == 2,
           "q must be [B, heads, D], k_cache [num_blocks, block_size, heads, D], block_table "
           "[B, max_blocks]");
@@ -196,6 +201,7 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
                      const OptTensor& scores, double decay, const OptTensor& out_arg,
                      const OptTensor& workspace_arg, const OptTensor& lam,
                      const OptTensor& norm_weight, double norm_eps, double out_scale) {
+  require_init();
   REQUIRE(q.dim() == 3 && unit(q, 2), "q must be [B, heads, D] with a unit inner stride");
   const Cache c = check_cache(k_cache, v_cache);
   const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), H = c.v_heads;
@@ -310,6 +316,7 @@ void append_tokens(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k
                    const Tensor& v_new, const Tensor& new_lens, const Tensor& seq_lens,
                    const Tensor& block_table, const OptTensor& scores, const OptTensor& positions,
                    const OptTensor& next_pos, const OptTensor& status) {
+  require_init();
   const Cache c = check_cache(k_cache, v_cache);
   REQUIRE(k_new.dim() == 4 && v_new.dim() == 4 && k_new.size(0) == v_new.size(0) &&
               k_new.size(1) == v_new.size(1) && k_new.size(2) == c.k_heads &&
@@ -361,6 +368,7 @@ void append_tokens(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k
 py::tuple select_evictions(const Tensor& scores, const Tensor& positions, const Tensor& seq_lens,
                            const Tensor& next_pos, int64_t budget, int64_t recent, int64_t sinks,
                            const std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>>& moves) {
+  require_init();
   REQUIRE(scores.dim() == 3, "scores must be [B, Hkv, T]");
   const int64_t B = scores.size(0), H = scores.size(1), T = scores.size(2);
   check_state(scores, "scores", kF32, B, H, 0, false);
@@ -415,6 +423,7 @@ py::tuple select_evictions(const Tensor& scores, const Tensor& positions, const 
 void compact_cache(const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table,
                    const Tensor& src, const Tensor& dst, const Tensor& counts,
                    const OptTensor& scores, const OptTensor& positions, const OptTensor& status) {
+  require_init();
   const Cache c = check_cache(k_cache, v_cache);
   REQUIRE(c.k_heads == c.v_heads, "k_cache and v_cache must have the same heads");
   const int64_t H = c.v_heads;

@@ -398,7 +398,8 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
     return BPT_ERR_INVALID_ARGUMENT;
   const int D = a->head_dim, width = maps * D;
   const int group = a->q_heads / a->kv_heads;
-  if (group > kMaxRows) return BPT_ERR_UNSUPPORTED_SHAPE;
+  if (group > kMaxRows || a->batch > 65535 || a->kv_heads > 65535)   // grid dimensions
+    return BPT_ERR_UNSUPPORTED_SHAPE;
   if (!(width == 64 || width == 128 || width == 256) || D < 64) return BPT_ERR_UNSUPPORTED_SHAPE;
   if (a->block_size < 16 || a->block_size > 256 || (a->block_size & (a->block_size - 1)))
     return BPT_ERR_UNSUPPORTED_SHAPE;

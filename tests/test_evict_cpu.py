@@ -122,6 +122,22 @@ def test_diff_refusals(match, kw):
                                          torch.zeros(1))
 
 
+def test_binding_without_its_library():
+    """The extension module alone, before bpt.evict gave it the library, refuses to work."""
+    import subprocess
+    import sys
+    code = ("import sys, torch; sys.path.insert(0, %r); import bpt._bind as b\n"
+            "t = torch.zeros(1, dtype=torch.int32)\n"
+            "try: b.compact_cache(t, t, t, t, t, t, None, None, None)\n"
+            "except RuntimeError as e: print('refused:', e)")
+    import bpt
+    import os
+    r = subprocess.run([sys.executable, "-c",
+                        code % os.path.dirname(os.path.dirname(bpt.__file__))],
+                       capture_output=True, text=True, timeout=300)
+    assert r.stdout.startswith("refused: bpt/_bind is used through"), r.stdout + r.stderr
+
+
 def test_diff_lambda_refusals():
     v = torch.zeros(64)
     with pytest.raises(BptArgumentError):
@@ -209,6 +225,7 @@ def decode_args(**kw):
     (_lib.ERR_UNSUPPORTED_SHAPE, dict(maps=2, head_dim=256, lam=0x100000)),
     (_lib.ERR_UNSUPPORTED_SHAPE, dict(block_size=8)),
     (_lib.ERR_UNSUPPORTED_SHAPE, dict(block_size=512)),
+    (_lib.ERR_UNSUPPORTED_SHAPE, dict(batch=65536)),
     (_lib.ERR_ALIGNMENT, dict(q=0x100002)), (0, dict(batch=0)),
 ])
 def test_abi_decode_refusals(status, kw):
