@@ -48,7 +48,8 @@ void bind_to(F& fn, const py::dict& table, const char* name) {
 }
 
 void require_init() {
-  if (__builtin_expect(!g_abi.compact, 0)) refuse("bpt/_bind is used through bpt.evict and bpt.diff");
+  if (__builtin_expect(!g_abi.compact, 0))
+    refuse("bpt/_bind is used through bpt.evict and bpt.diff");
 }
 
 // The message is built only for a call that is refused.

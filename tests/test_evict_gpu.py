@@ -134,6 +134,44 @@ def test_scored_repeats_bitwise_and_by_graph():
                           (sa - 0.5 * start)[0, :, :900], rtol=1e-5, atol=1e-7)
 
 
+def test_scored_two_streams_and_two_graphs_at_once():
+    """Calls that overlap on two streams, eager and captured, each with its own workspace, give what
+    they give alone."""
+    from bpt import evict
+    cases = [attend_case(30 + i, lens, 8, 2, 128, 16, FP16)
+             for i, lens in enumerate(([3000, 5], [2000, 1999, 64]))]
+    run = lambda c, s: evict.paged_decode_attention_scored(  # noqa: E731
+        c["q"], c["k"], c["v"], c["bt"], c["sl"], s, decay=0.0)
+    alone = []
+    for c in cases:
+        s = c["scores"].clone()
+        alone.append((run(c, s).clone(), s))
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs, held = [], []
+    for c, st in zip(cases, streams):
+        s = c["scores"].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = run(c, s)
+        graphs.append(g)
+        held.append((out, s))
+    torch.cuda.synchronize()
+    for turn in range(20):
+        got = []
+        for c, st, g, h in zip(cases, streams, graphs, held):
+            with torch.cuda.stream(st):
+                if turn % 2:
+                    s = c["scores"].clone()
+                    got.append((run(c, s), s))
+                else:
+                    h[1].copy_(c["scores"])
+                    g.replay()
+                    got.append(h)
+        torch.cuda.synchronize()
+        for a, b in zip(got, alone):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_scored_far_pages():
     """Pages past 2^31 elements of a cache (4.5 GB each)."""
     from bpt import evict
