@@ -35,9 +35,10 @@ constexpr int kFinishThreads = kFinishWarps * 32;
 constexpr int kScoreTokens = 4 * kFinishThreads;  // tokens of a round of a scoring CTA
 constexpr int kMaxRows = 8;                       // q rows per kv head
 static_assert(kMaxRows >= kFinishWarps, "shared rows double as one value a warp");
-// Scoring CTAs an SM, each of several rounds: 29 us for 59 MB of logits with a CTA per 1024
-// tokens (B=16, 24-32k tokens, 32 q heads), 20 us with 4 an SM; 8 measured as 4.
-constexpr int kScoreCtas = 4;
+// Scoring CTAs an SM, as many as fit at once, each of several rounds: 29 us for 59 MB of logits
+// with a CTA per 1024 tokens (B=16, 24-32k tokens, 32 q heads), 20 us with 3 or 4 an SM; the whole
+// call at B=8, 12-16k tokens 81.4 us with 3 (two rounds), 82.4 with 4 and more (one).
+constexpr int kScoreCtas = 3;
 // The logits stay in L2 (evict-last stores). A buffer that would be written back while the next
 // call streams its cache is dropped line by line once read: 306 -> 298 us at 59 MB, 627 -> 620
 // at 114 MB (B=16). At 17 MB dropping costs more than it saves: 89 -> 92 us (B=1, 128k tokens).
