@@ -44,14 +44,15 @@ constexpr int kScoreCtas = 3;
 // at 114 MB (B=16). At 17 MB dropping costs more than it saves: 89 -> 92 us (B=1, 128k tokens).
 constexpr int64_t kDropBytes = 32 << 20;
 
-// Split CTA shape: 2 warps of 16 tokens each, a 3-stage ring, and as many CTAs an SM as the ring
-// of a width allows (4 at 128 channels, 2 at 256). Width 256 measured with 64-token chunks in 2
-// stages and 1 CTA: 107 us; 32-token chunks, 3 CTAs of 2 stages (registers spill): 100 us; 2 CTAs
-// of 3 stages: 84 us (differential, B=8, 16k tokens, 4 value heads of 256).
+// Split CTA shape: 2 warps of 16 tokens each, and as many stages and CTAs an SM as keep about
+// 200 KB of cache on its way: 160 (registers allow no more), 192 and 192 KB at 64, 128 and 256
+// channels. Measured at B=8 and 0.47 GB of cache: width 64 with 3 stages and 4 CTAs 94 us, 4 and 5
+// 89.5, 4 and 6 96.5, 6 and 4 92.6; width 256 with 64-token chunks in 2 stages and 1 CTA 107 us,
+// 32-token chunks in 2 stages and 3 CTAs (registers spill) 100, 3 and 2 84.
 constexpr int kSplitWarps = 2;
-constexpr int kStages = 3;
 constexpr int kChunk = 16 * kSplitWarps;
-constexpr int resident_ctas(int width) { return width >= 256 ? 2 : 4; }
+constexpr int stages(int width) { return width == 64 ? 4 : 3; }
+constexpr int resident_ctas(int width) { return width >= 256 ? 2 : width >= 128 ? 4 : 5; }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
@@ -299,11 +300,11 @@ finish_scored_kernel(const FinishParams p) {
 template <int D, bool BF16, bool DIFF>
 int launch_both(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeParams& p,
                 const FinishParams& f, cudaStream_t st) {
-  constexpr int R = resident_ctas(D);
+  constexpr int R = resident_ctas(D), N = stages(D);
   using Op = mma::OpState<BF16, DIFF>;
   const bool wide = p.group > 4;
-  const int rc = wide ? mma::launch<D, kSplitWarps, kStages, R, true, Op>(tk, tv, p, st)
-                      : mma::launch<D, kSplitWarps, kStages, R, false, Op>(tk, tv, p, st);
+  const int rc = wide ? mma::launch<D, kSplitWarps, N, R, true, Op>(tk, tv, p, st)
+                      : mma::launch<D, kSplitWarps, N, R, false, Op>(tk, tv, p, st);
   if (rc) return rc;
   const int64_t grid = int64_t(f.n_merge) +
                        (f.scores ? int64_t(p.batch) * p.kv_heads * f.parts : 0);
@@ -348,8 +349,8 @@ ScoredView scored_view(void* ws, int batch, int rows, int width, int splits, int
 }
 
 // The shared planner's count, but one chunk a split where that still is one wave (the planner
-// keeps two): B=1, 8 kv heads of 128, 512 / 1024 / 2048 tokens 6.3 / 6.6 / 7.5 us against 7.1 / 7.5 /
-// 8.1 with two.
+// keeps two): B=1, 8 kv heads of 128, 512 / 1024 / 2048 tokens 6.3 / 6.6 / 7.5 us against 7.1 / 7.5
+// / 8.1 with two (5.9 / 6.3 / 7.2 now).
 int state_splits(int width, int batch, int kv_heads, int block_size, int max_blocks,
                  int num_splits, int sm_count) {
   const int resident = resident_ctas(width);

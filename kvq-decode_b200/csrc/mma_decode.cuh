@@ -250,7 +250,15 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     const int32_t* bt = p.block_table + int64_t(b) * p.bt_sb;
     const int R = p.box_rows;                     // min(block_size, CHUNK)
     const int bs = p.block_size;
+    const int bs_shift = __ffs(bs) - 1;           // a power of two
     const uint32_t box_bytes = uint32_t(R) * 64 * 2;
+    // OpState issues the boxes of a chunk with a lane each, instead of one after the other: in the
+    // first STAGES + 1 chunks, all that short splits have (B=1, 4k / 8k tokens of 128 channels: 8.8
+    // -> 8.1, 11.5 -> 9.8 us), and throughout where boxes are many or small (B=8, 0.47 GB: 130 ->
+    // 89 us at 64 channels, 92 -> 81 us at 256 channels in pages of 16). Elsewhere the paced stream
+    // of one lane is 2 % faster (B=4, 64k tokens of 128 channels: 174 against 178 us): it stays.
+    static_assert(!Op::kState || (CHUNK / 16) * 2 * C::NCB <= 32, "a lane per box of a chunk");
+    const bool many_boxes = D == 64 || CHUNK / R * C::NCB >= 8;
     const int last_page = (t_end - 1) / bs;
     int win_base = t_begin / bs;                  // lane i caches block_table[win_base + i]
     int win = (win_base + lane <= last_page) ? __ldg(bt + win_base + lane) : 0;
@@ -258,8 +266,9 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     for (int c = 0; c < nchunks; ++c) {
       const int stage = c % STAGES;
       const uint32_t par = uint32_t(c / STAGES) & 1u;
-      bool w_ok = (lane == 0) ? mbar_wait(&empty[stage], par ^ 1u) : true;
-      w_ok = __shfl_sync(kFullMask, w_ok, 0);
+      const bool at_once = Op::kState && (many_boxes || c <= STAGES);
+      bool w_ok = (lane == 0 || at_once) ? mbar_wait(&empty[stage], par ^ 1u) : true;
+      w_ok = Op::kState ? bool(__all_sync(kFullMask, w_ok)) : __shfl_sync(kFullMask, w_ok, 0);
       if (!w_ok) {
         if (lane == 0) flag_device_error(p.status, BPT_DEV_WAIT_TIMEOUT);
         break;
@@ -268,6 +277,37 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       const int nbox = min(CHUNK / R, cdiv(t_end - tok0, R));
       if (lane == 0)
         mbar_arrive_expect_tx(&full[stage], uint32_t(nbox) * C::NCB * box_bytes * 2u);
+      if (at_once) {
+        // a lane per box: page j of the chunk, 64-column block cb, K or V
+        const int j = lane / (2 * C::NCB), cb = (lane >> 1) % C::NCB;
+        const int pg_first = tok0 >> bs_shift, pg_last = (tok0 + (nbox - 1) * R) >> bs_shift;
+        if (pg_last - win_base >= 32) {          // warp-uniform
+          win_base = pg_first;
+          win = (win_base + lane <= last_page) ? __ldg(bt + win_base + lane) : 0;
+        }
+        const int t = tok0 + j * R, pg = t >> bs_shift;
+        int phys = __shfl_sync(kFullMask, win, min(pg - win_base, 31));
+        if (j < nbox) {
+          if (phys < 0 || int64_t(phys) >= p.num_blocks) {
+            flag_device_error(p.status, BPT_DEV_BAD_BLOCK_ID);
+            phys = 0;
+          }
+          const int row = t - (pg << bs_shift);
+          const int so = stage * C::STAGE_ELEMS + cb * C::BLOCK_ELEMS + j * R * 64;
+          if (lane & 1) {
+            tma_load_4d(sV + so, &tmV, &full[stage], cb * 64, p.v_c1 ? row : h,
+                        p.v_c1 ? h : row, phys, pol);
+          } else {
+            // DIFF: the first half of the columns is key head 2h, the second key head 2h + 1
+            const int kcol = Op::kDiff ? cb * 64 % (D / 2) : cb * 64;
+            const int kh = Op::kDiff ? 2 * h + cb * 64 / (D / 2) : h;
+            tma_load_4d(sK + so, &tmK, &full[stage], kcol, p.k_c1 ? row : kh,
+                        p.k_c1 ? kh : row, phys, pol);
+          }
+        }
+        ++issued;
+        continue;
+      }
       for (int j = 0; j < nbox; ++j) {
         const int t = tok0 + j * R;
         const int pg = t / bs;

@@ -255,8 +255,8 @@ def test_abi_decode_workspace():
 
 
 def test_abi_decode_splits():
-    """One 32-token chunk a split while that is one wave of 4 (width 256: 2) CTAs an SM, else the
-    decode planner's count; requests are clamped to the chunks."""
+    """One 32-token chunk a split while that is one wave of 4 (width 64: 5, 256: 2) CTAs an SM, else
+    the decode planner's count; requests are clamped to the chunks."""
     f = _lib.lib().bpt_effective_splits_scored
     plan = _lib.lib().bpt_plan_splits
 
@@ -268,6 +268,7 @@ def test_abi_decode_splits():
     assert splits(128, 1, 64, 8, 16, 4096, 0, 148) == plan(64, 8, 16, 4096, 148)
     assert splits(128, 2, 1, 8, 16, 128, 0, 148) == 32      # 512 CTAs of one chunk are 2 waves
     assert splits(128, 2, 8, 4, 32, 512, 0, 148) == 9       # 2 CTAs an SM: 296 / 32
+    assert splits(64, 1, 1, 8, 16, 184, 0, 148) == 92       # 736 of 740 CTAs
     assert splits(128, 1, 2, 8, 16, 4, 7, 148) == 2
     assert splits(128, 1, 1, 8, 16, 0, 0, 148) == 1
 
