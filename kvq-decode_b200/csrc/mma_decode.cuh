@@ -258,7 +258,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     // 89 us at 64 channels, 92 -> 81 us at 256 channels in pages of 16). Elsewhere the paced stream
     // of one lane is 2 % faster (B=4, 64k tokens of 128 channels: 174 against 178 us): it stays.
     static_assert(!Op::kState || (CHUNK / 16) * 2 * C::NCB <= 32, "a lane per box of a chunk");
-    const bool many_boxes = D == 64 || CHUNK / R * C::NCB >= 8;
+    bool many_boxes = CHUNK / R * C::NCB >= 8;
+    if (D == 64) many_boxes = true;
     const int last_page = (t_end - 1) / bs;
     int win_base = t_begin / bs;                  // lane i caches block_table[win_base + i]
     int win = (win_base + lane <= last_page) ? __ldg(bt + win_base + lane) : 0;
