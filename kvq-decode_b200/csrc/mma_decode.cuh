@@ -127,12 +127,11 @@ __device__ __forceinline__ void mma_16816_zc(float (&d)[4], uint32_t a0, uint32_
 // in fp32 round-to-nearest: a long-running accumulator never passes through the tensor
 // core's own accumulation, whose per-step rounding would otherwise build up over thousands
 // of tokens on a large running sum.
-template <bool BF16 = false>
 __device__ __forceinline__ void mma_16816_acc(float (&acc)[4], uint32_t a0, uint32_t a1,
                                               uint32_t a2, uint32_t a3, uint32_t b0,
                                               uint32_t b1) {
   float t[4];
-  mma_16816_zc<BF16>(t, a0, a1, a2, a3, b0, b1);
+  mma_16816_zc(t, a0, a1, a2, a3, b0, b1);
   acc[0] += t[0]; acc[1] += t[1]; acc[2] += t[2]; acc[3] += t[3];
 }
 
@@ -142,22 +141,27 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 }
 
 // hi = fp16(p) and lo = fp16(p - hi) for two adjacent tokens, packed as half2: ~22 bits of p.
-// With bf16 (whose MMA takes bf16 operands only) the pair carries ~16 bits, a relative error
-// of at most 2^-17 in a weight whose output is rounded to bf16 (2^-9).
-template <bool BF16 = false>
 __device__ __forceinline__ void split_hi_lo(float p0, float p1, uint32_t& hi, uint32_t& lo) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
-    const float2 hf = __bfloat1622float2(h);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(p0 - hf.x, p1 - hf.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-    return;
-  }
   __half2 h = __floats2half2_rn(p0, p1);
   const float2 hf = __half22float2(h);
   hi = *reinterpret_cast<uint32_t*>(&h);
   lo = pack_half2(p0 - hf.x, p1 - hf.y);
+}
+
+// p = hi + mid + lo in bf16 (a bf16 MMA takes no other operand), exactly: each remainder is exact,
+// and 3 x 8 bits hold fp32's 24. Two limbs (a relative error of up to 2^-17) put 1 in 200 outputs of
+// a normalised differential layer one bf16 step beside what fp32 weights give.
+__device__ __forceinline__ void split_bf16(float p0, float p1, uint32_t& hi, uint32_t& mid,
+                                           uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);
+  const float2 hf = __bfloat1622float2(h);
+  const float r0 = p0 - hf.x, r1 = p1 - hf.y;
+  const __nv_bfloat162 m = __floats2bfloat162_rn(r0, r1);
+  const float2 mf = __bfloat1622float2(m);
+  const __nv_bfloat162 l = __floats2bfloat162_rn(r0 - mf.x, r1 - mf.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  mid = *reinterpret_cast<const uint32_t*>(&m);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 __device__ __forceinline__ void fence_proxy_async_smem() {
@@ -453,9 +457,15 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     const float p0 = fast_exp2(x0 - m_use), p1 = fast_exp2(x1 - m_use);
     const float p2 = fast_exp2(x2 - m_use), p3 = fast_exp2(x3 - m_use);
     l_run += (p0 + p1) + (p2 + p3);
-    uint32_t hi0, lo0, hi1, lo1;
-    split_hi_lo<Op::kBf16>(p0, p1, hi0, lo0);
-    split_hi_lo<Op::kBf16>(p2, p3, hi1, lo1);
+    // fp16: hi + lo; bf16: hi + lo + low
+    uint32_t hi0, lo0, hi1, lo1, low0 = 0u, low1 = 0u;
+    if constexpr (Op::kBf16) {
+      split_bf16(p0, p1, hi0, lo0, low0);
+      split_bf16(p2, p3, hi1, lo1, low1);
+    } else {
+      split_hi_lo(p0, p1, hi0, lo0);
+      split_hi_lo(p2, p3, hi1, lo1);
+    }
 
     // ---- rows past the end of the split: zero V so stale or NaN bytes cannot reach O
     if (lim < 16) {
@@ -472,25 +482,33 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     // ---- O^T += V^T P^T
     const uint32_t pb0 = G8 ? hi0 : (g < 4 ? hi0 : lo0);
     const uint32_t pb1 = G8 ? hi1 : (g < 4 ? hi1 : lo1);
+    if constexpr (Op::kBf16 && !G8) {              // columns 0-3, one lane group of 4 a column
+      low0 = g < 4 ? low0 : 0u;
+      low1 = g < 4 ? low1 : 0u;
+    }
 #pragma unroll
     for (int db = 0; db < C::DB16; ++db) {
       const uint32_t chunk = (uint32_t((2 * db) & 7) | ld_sel) ^ ld_swz;
       const uint32_t addr = vbase + uint32_t(db >> 2) * C::BLOCK_BYTES + ld_row + (chunk << 4);
       uint32_t a0, a1, a2, a3;
       ldsm_x4_trans(addr, a0, a1, a2, a3);
-      if constexpr (G8 && Op::kState) {
-        // hi and lo products of one tile meet in the tensor core, the tiles in fp32: half of
-        // the accumulator registers (168 + spills against none at D = 128)
+      if constexpr (Op::kState && (G8 || Op::kBf16)) {
+        // the limbs' products of one tile meet in the tensor core, smallest first, and the tiles
+        // in fp32: with G8 half of the accumulator registers of one accumulator a limb
         float t[4];
-        mma_16816_zc<Op::kBf16>(t, a0, a1, a2, a3, hi0, hi1);
-        mma_16816<Op::kBf16>(t, a0, a1, a2, a3, lo0, lo1);
+        if constexpr (Op::kBf16) {
+          mma_16816_zc<true>(t, a0, a1, a2, a3, low0, low1);
+          if constexpr (G8) mma_16816<true>(t, a0, a1, a2, a3, lo0, lo1);
+        } else {
+          mma_16816_zc(t, a0, a1, a2, a3, lo0, lo1);
+        }
+        mma_16816<Op::kBf16>(t, a0, a1, a2, a3, pb0, pb1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[0][db][e] += t[e];
         continue;
       }
-      mma_16816_acc<Op::kBf16>(acc[0][db], a0, a1, a2, a3, pb0, pb1);
-      if constexpr (G8)
-        mma_16816_acc<Op::kBf16>(acc[C::NACC - 1][db], a0, a1, a2, a3, lo0, lo1);
+      mma_16816_acc(acc[0][db], a0, a1, a2, a3, pb0, pb1);
+      if constexpr (G8) mma_16816_acc(acc[C::NACC - 1][db], a0, a1, a2, a3, lo0, lo1);
     }
     if (lim < 16) fence_proxy_async_smem();
     __syncwarp();
