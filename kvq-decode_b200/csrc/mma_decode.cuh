@@ -54,6 +54,13 @@ struct OpState {
   static constexpr bool kBf16 = BF16, kState = true, kDiff = DIFF;
 };
 
+// OpState's fp16 weights, at most 1, meet the values 2^15 times as large (exact, taken back from
+// the sums). fp16's smallest step is 2^-24: unscaled, weights below 2^-14 of the warp's maximum
+// lost bits, and those below 2^-25 were 0 beside the values while the softmax sum counted them.
+// A sink 17 nats above the other tokens made their share of the output 20 % wrong. Scaled, a
+// weight is off by at most 2^-22 of itself or 2^-40 of the maximum.
+constexpr float kWeightScale = 32768.f;
+
 template <int D, int NCW, int STAGES, bool G8, typename Op = OpFp16>
 struct Cfg {
   static constexpr int CHUNK = 16 * NCW;              // tokens per stage
@@ -463,8 +470,9 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       split_bf16(p0, p1, hi0, lo0, low0);
       split_bf16(p2, p3, hi1, lo1, low1);
     } else {
-      split_hi_lo(p0, p1, hi0, lo0);
-      split_hi_lo(p2, p3, hi1, lo1);
+      constexpr float kUp = Op::kState ? kWeightScale : 1.f;
+      split_hi_lo(p0 * kUp, p1 * kUp, hi0, lo0);
+      split_hi_lo(p2 * kUp, p3 * kUp, hi1, lo1);
     }
 
     // ---- rows past the end of the split: zero V so stale or NaN bytes cannot reach O
@@ -530,6 +538,7 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
       } else {
         acc[0][i][e] += __shfl_xor_sync(kFullMask, acc[0][i][e], 2);
       }
+      if constexpr (Op::kState && !Op::kBf16) acc[0][i][e] *= 1.f / kWeightScale;
     }
   named_barrier_sync(1, NCW * 32);  // every consumer warp is done reading the ring
   if (t4 == 0 && (G8 || g < 4)) {

@@ -9,8 +9,9 @@ arithmetic and not from a run:
     scale is one more product: |dx| <= (D / 16 + 3) * 2^-21 * scale * sum |q_i k_i|.
   * a weight is 2^(x - m) / L: relative error |dx| (numerator) + |dx| (sum) + 16 roundings of 2^-23
     (two exponentials of 2 ulp each, the joins of warps and splits, the quotient) + the precision
-    of a weight on its way to the values: 2^-21 for fp16 pairs; the three bf16 limbs are exact
-    (2^-16, which a pair of them would have, is a bound with room).
+    of a weight on its way to the values: 2^-21 for fp16 pairs (or 2^-40 of the largest weight,
+    where that is more: `tests/test_evict_weights_gpu.py`); the three bf16 limbs are exact, and
+    2^-16, which a pair of them would have, is a bound with room.
   * a value product then adds at most its weights' errors times |v|, and fp32 sums of the
     partial products: one tile per 16 tokens, joined pairwise by warps and splits; the running
     sum of n / 32 tiles rounds at 2^-24 of its magnitude each time, in a random walk:

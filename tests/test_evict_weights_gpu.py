@@ -70,3 +70,46 @@ def test_bf16_weights_keep_fp32_precision(G, maps):
         d = np.arange(r, width, G)
         want = (rest[:, r] / L[:, r])[:, None]
         assert (np.abs(got[:, j, d] - want) * L[:, r][:, None] <= 2.0 ** -19.2).all()
+
+
+@pytest.mark.parametrize("G", [1, 4, 8])
+@pytest.mark.parametrize("maps", [1, 2])
+def test_fp16_tail_beside_a_sink(G, maps):
+    """One token far above all the others, whose value is 0: the output is what the others, each of
+    a tiny weight, leave. All in one split, so that the sink's warp holds half of them.
+
+    The logits are single exact products as above, |x| <= 32 in log2: 2^-23 * 32 ln 2 of error in a
+    weight, and 2^-22 of the exponential: below 2^-18.4. A weight is carried with 2^-22 of itself or
+    2^-40 of the sink's. The sum of n equal terms adds sqrt(n) 2^-23, the joins 2^-20, the output's
+    rounding 2^-11 of itself (nothing is below fp16's normal range)."""
+    if maps == 2 and G % 2:
+        G += 1
+    from bpt import diff, evict
+    n, D = 2000, 64
+    nats = [4, 8, 12, 14, 17, 20]
+    B, width = len(nats), maps * D
+    c = attend_case(G, [n] * B, G, 1, D, 16, FP16, maps=maps)
+    c["q"].zero_()
+    c["q"][:, :, 0] = 1.0
+    c["k"].zero_()
+    c["v"].fill_(200.0)
+    for b, x in enumerate(nats):
+        pages = c["bt"][b, :n // 16].long()
+        c["k"][pages, :, :, 0] = -8.0 * x
+        c["k"][pages[0], 0] = 0.0
+        c["v"][pages[0], 0] = 0.0
+    if maps == 1:
+        out = evict.paged_decode_attention_scored(c["q"], c["k"], c["v"], c["bt"], c["sl"],
+                                                  c["scores"], num_splits=1)
+    else:
+        out = diff.paged_decode_attention_diff(c["q"], c["k"], c["v"], c["bt"], c["sl"],
+                                               torch.zeros(G // 2, device="cuda"), num_splits=1)
+    e = np.exp(-np.array(nats, np.float64))
+    L = 1.0 + (n - 1) * e
+    want = (n - 1) * e * 200.0 / L
+    tol = want * (2.0 ** -18.4 + 2.0 ** -22 + np.sqrt(n) * 2.0 ** -23 + 2.0 ** -20) + \
+        (n - 1) * 2.0 ** -40 * 200.0 / L
+    got = f64(out).reshape(B, -1)
+    assert want.min() > 2.0 ** -13
+    worst = np.abs(got - want[:, None]).max(axis=1)
+    assert (worst <= tol + (want + tol) * 2.0 ** -11).all(), worst / want
