@@ -205,8 +205,8 @@ enum bpt_dtype { BPT_FP16 = 1, BPT_BF16 = 2 };
  * maps 2, the differential decode: q [B, 2 H, D], k_cache [.., 2 Hkv, D], v_cache
  *   [.., Hkv, 2 D], out [B, H, 2 D]; H / Hkv <= 4; D 64 or 128. q_heads is 2 H. Output head j is
  *   (softmax(q_2j.k_2h) - lam_j softmax(q_2j+1.k_2h+1)) v_h, h = j / (H / Hkv); where norm_weight
- *   [2 D] is set it is divided by sqrt(mean square + norm_eps) and multiplied by the weight;
- *   then by out_scale. The score adds the sum of |weight of map 1 - lam_j weight of map 2|.
+ *   [2 D] is set it is divided by sqrt(mean square + norm_eps) and multiplied by the weight (a
+ *   row whose fp32 mean square is 0 gives zeros, norm_eps 0 included); then by out_scale. The score adds the sum of |weight of map 1 - lam_j weight of map 2|.
  * q, caches and out are fp16 or bf16; scores, lam and norm_weight fp32. Softmax, sums and
  * scores are fp32. An empty sequence gives zeros. decay 0 ignores the old scores (NaN among
  * them); slots past a sequence's end keep theirs. Keys must be finite with maps 2. */

@@ -192,7 +192,8 @@ __device__ __forceinline__ void join_output(const FinishParams& p, int id, float
     float total = 0.f;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) total += s_red[k];
-    mul *= rsqrtf(total / float(D) + p.norm_eps) * w;
+    // a row of zeros (an empty sequence is one) stays zeros with norm_eps 0 too
+    mul *= total == 0.f ? 0.f : rsqrtf(total / float(D) + p.norm_eps) * w;
   }
   if (tid < D)
     store16<BF16>(p.out, int64_t(b) * p.o_sb + int64_t(j) * p.o_sh + tid, DIFF ? r * mul : r);
