@@ -187,6 +187,9 @@ int64_t scored_workspace_bytes(int maps, const Tensor& q, const Tensor& k_cache,
   REQUIRE(q.dim() == 3 && k_cache.dim() == 4 && block_table.dim() == 2,
           "q must be [B, heads, D], k_cache [num_blocks, block_size, heads, D], block_table "
           "[B, max_blocks]");
+  REQUIRE(maps == 1 || maps == 2, "maps must be 1 (scored) or 2 (differential)");
+  REQUIRE(k_cache.size(2) > 0 && k_cache.size(2) % maps == 0 && q.size(1) > 0 && q.size(2) > 0,
+          "k_cache must have maps heads for each kv head, q heads and channels");
   const int B = int(q.size(0)), Hq = int(q.size(1)), D = int(q.size(2));
   const int bs = int(k_cache.size(1)), mb = int(block_table.size(1));
   const c10::cuda::OptionalCUDAGuard guard(q.is_cuda() ? c10::optional<c10::Device>(q.device())
