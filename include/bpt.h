@@ -214,7 +214,8 @@ typedef struct bpt_scored_decode {
   int dtype, maps;
   int batch, q_heads, kv_heads, head_dim, block_size, max_blocks;
   int num_splits, sm_count;                          /* as bpt_decode_fp16 */
-  float scale, decay, norm_eps, out_scale;           /* scale <= 0: 1 / sqrt(head_dim) */
+  float scale, decay, norm_eps, out_scale;           /* scale <= 0: 1 / sqrt(head_dim); the
+                                                      * first three finite, norm_eps >= 0 */
   int64_t num_blocks;
   const void* q;        int64_t q_stride[2];         /* batch, head */
   const void* k_cache;  int64_t k_stride[3];         /* block, token, head */

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cfloat>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -221,8 +222,10 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
   REQUIRE(cap <= INT32_MAX && B <= 65535, "more than 2^31 slots or 65535 sequences");
   const int64_t out_heads = Hq / maps;
   if (scores) check_state(*scores, "scores", kF32, B, H, cap, true);
-  REQUIRE(std::isfinite(decay) && decay >= 0.0, "decay must be finite and not negative");
-  REQUIRE(!scale || (std::isfinite(*scale) && *scale > 0.0), "scale must be positive and finite");
+  // as the kernels take them: a scale that is 0 in fp32 would mean the default one
+  REQUIRE(std::isfinite(float(decay)) && decay >= 0.0, "decay must be finite and not negative");
+  REQUIRE(!scale || (float(*scale) > 0.f && float(*scale) <= FLT_MAX / 2),
+          "scale must be positive and finite in fp32");
   if (maps == 2) {
     REQUIRE(lam && lam->scalar_type() == kF32 &&
                 ((lam->dim() == 1 && lam->size(0) == out_heads) ||
@@ -231,7 +234,8 @@ Tensor decode_scored(int maps, const Tensor& q, const Tensor& k_cache, const Ten
     REQUIRE(!norm_weight || (norm_weight->dim() == 1 && norm_weight->size(0) == width &&
                              norm_weight->scalar_type() == kF32 && unit(*norm_weight, 0)),
             "norm_weight must be contiguous float32 " + dims({width}));
-    REQUIRE(norm_eps >= 0.0, "norm_eps must not be negative");
+    REQUIRE(norm_eps >= 0.0 && std::isfinite(float(norm_eps)),
+            "norm_eps must be finite and not negative");
   }
   const Device on(q);
   on.same(k_cache, "k_cache");

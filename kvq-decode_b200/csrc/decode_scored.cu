@@ -18,6 +18,7 @@
 // reading the keys again would cost 2 D a kv head and token.
 #include <cuda_bf16.h>
 #include <cudaTypedefs.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -400,6 +401,10 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
     return BPT_ERR_INVALID_ARGUMENT;
   if (a->batch < 0 || a->kv_heads <= 0 || a->q_heads <= 0 || a->q_heads % (maps * a->kv_heads) ||
       a->block_size <= 0 || a->max_blocks < 0 || a->num_blocks < 0 || a->head_dim <= 0)
+    return BPT_ERR_INVALID_ARGUMENT;
+  // log2(e) * scale and the products with decay and norm_eps have to be numbers
+  if (!(a->scale <= FLT_MAX / 2) || (a->scores && !(fabsf(a->decay) <= FLT_MAX)) ||
+      (maps == 2 && a->norm_weight && !(a->norm_eps >= 0.f && a->norm_eps <= FLT_MAX)))
     return BPT_ERR_INVALID_ARGUMENT;
   if (a->batch == 0) return BPT_OK;
   if (!a->q || !a->k_cache || !a->v_cache || (!a->block_table && a->max_blocks > 0) ||

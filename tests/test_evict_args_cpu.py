@@ -1,8 +1,18 @@
 """Arguments at the border of what the scored decode and the eviction accept: refused with an error
 before anything is launched."""
+import ctypes
 import os
 import subprocess
 import sys
+
+import pytest
+import torch
+
+from bpt import BptArgumentError, _lib, diff
+from test_evict_cpu import decode_args, scored, tensors
+
+c_vp = ctypes.c_void_p
+FLOAT_MAX = torch.finfo(torch.float32).max
 
 
 def test_workspace_of_an_operator_that_does_not_exist():
@@ -26,3 +36,54 @@ def test_workspace_of_an_operator_that_does_not_exist():
                        capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stderr)
     assert r.stdout.count("refused:") == 7, r.stdout
+
+
+@pytest.mark.parametrize("scale", [1e-50, 1e39, FLOAT_MAX])
+def test_scale_that_fp32_cannot_hold(scale):
+    """1e-50 is 0 in fp32, which the C ABI takes for the default; log2(e) of the largest is infinite."""
+    with pytest.raises(BptArgumentError, match="scale"):
+        scored(tensors(), scale=scale)
+    t = tensors(maps=2)
+    with pytest.raises(BptArgumentError, match="scale"):
+        diff.paged_decode_attention_diff(t["q"], t["k"], t["v"], t["bt"], t["sl"],
+                                         torch.zeros(2), scale=scale)
+
+
+def test_small_scale_is_no_error():
+    with pytest.raises(BptArgumentError, match="no CPU"):
+        scored(tensors(), scale=1e-40)
+
+
+@pytest.mark.parametrize("decay", [1e39, 1e300])
+def test_decay_that_fp32_cannot_hold(decay):
+    with pytest.raises(BptArgumentError, match="decay"):
+        scored(tensors(), decay=decay)
+
+
+@pytest.mark.parametrize("eps", [1e39, float("inf"), float("nan")])
+def test_norm_eps_that_fp32_cannot_hold(eps):
+    t = tensors(maps=2)
+    with pytest.raises(BptArgumentError, match="norm_eps"):
+        diff.paged_decode_attention_diff(t["q"], t["k"], t["v"], t["bt"], t["sl"], torch.zeros(2),
+                                         norm_weight=torch.ones(128), norm_eps=eps)
+
+
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("status,kw", [
+    (_lib.ERR_INVALID_ARGUMENT, dict(scale=NAN)), (_lib.ERR_INVALID_ARGUMENT, dict(scale=INF)),
+    (_lib.ERR_INVALID_ARGUMENT, dict(scale=FLOAT_MAX)),
+    (_lib.ERR_INVALID_ARGUMENT, dict(scores=0x300000, decay=NAN)),
+    (_lib.ERR_INVALID_ARGUMENT, dict(scores=0x300000, decay=INF)),
+    (_lib.ERR_INVALID_ARGUMENT, dict(maps=2, lam=0x300000, norm_weight=0x310000, norm_eps=NAN)),
+    (_lib.ERR_INVALID_ARGUMENT, dict(maps=2, lam=0x300000, norm_weight=0x310000, norm_eps=-1.0)),
+    # what is not used is not looked at: these get as far as the workspace
+    (_lib.ERR_WORKSPACE_TOO_SMALL, dict(scale=-1.0)), (_lib.ERR_WORKSPACE_TOO_SMALL,
+                                                       dict(decay=NAN)),
+    (_lib.ERR_WORKSPACE_TOO_SMALL, dict(maps=2, lam=0x300000, norm_eps=NAN)),
+])
+def test_abi_numbers(status, kw):
+    rc = _lib.lib().bpt_decode_scored(ctypes.byref(decode_args(**kw)), c_vp(0x200000),
+                                      ctypes.c_size_t(16), None)
+    assert rc == status
