@@ -624,6 +624,25 @@ CacheView view_of(void* base, const int64_t* stride, int dim) {
   return v;
 }
 
+struct Range {
+  uintptr_t lo, hi;         // addresses, hi past the end
+  bool meets(const Range& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+Range words(const void* p, int64_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  return {a, a + uintptr_t(n) * 4};
+}
+
+// What rows [batch, heads, slots] of state can reach.
+Range state_words(const void* p, int64_t sb, int64_t sh, int batch, int heads, int slots) {
+  if (!p || slots == 0) return {0, 0};
+  const int64_t b = sb * (batch - 1), h = sh * (heads - 1);
+  const char* base = static_cast<const char*>(p);
+  return {reinterpret_cast<uintptr_t>(base + 4 * ((b < 0 ? b : 0) + (h < 0 ? h : 0))),
+          reinterpret_cast<uintptr_t>(base + 4 * ((b > 0 ? b : 0) + (h > 0 ? h : 0) + slots))};
+}
+
 bool vec16(const CacheView& v) {
   return (reinterpret_cast<uintptr_t>(v.base) | uintptr_t(v.sb) | uintptr_t(v.st) |
           uintptr_t(v.sh) | uintptr_t(v.row_bytes)) % 16 == 0;
@@ -661,10 +680,20 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
       int64_t(recent) + sinks > budget)
     return BPT_ERR_INVALID_ARGUMENT;
   if (batch == 0) return BPT_OK;
-  if (!seq_lens || !next_pos || !src || !dst || !counts || !new_lens || seq_lens == new_lens ||
+  if (!seq_lens || !next_pos || !src || !dst || !counts || !new_lens ||
       (slots > 0 && (!scores || !positions)))
     return BPT_ERR_INVALID_ARGUMENT;
   const int64_t rows = int64_t(batch) * kv_heads;
+  // one CTA writes what others of the row have still to read: no result may lie on an input, nor
+  // on another result
+  const int64_t moves = bpt_evict_moves(budget, slots);
+  const Range range[8] = {words(src, rows * moves), words(dst, rows * moves), words(counts, rows),
+                          words(new_lens, batch), words(seq_lens, batch), words(next_pos, batch),
+                          state_words(scores, sc_sb, sc_sh, batch, kv_heads, slots),
+                          state_words(positions, pos_sb, pos_sh, batch, kv_heads, slots)};
+  for (int i = 0; i < 4; ++i)
+    for (int j = i + 1; j < 8; ++j)
+      if (range[i].meets(range[j])) return BPT_ERR_INVALID_ARGUMENT;
   if (rows > INT32_MAX / kMaxCluster) return BPT_ERR_UNSUPPORTED_SHAPE;
   const int C = cluster_size(rows, slots, device_sm_count());
   SelectParams p{};
@@ -683,7 +712,7 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   p.sinks = sinks;
   p.src = src;
   p.dst = dst;
-  p.moves = bpt_evict_moves(budget, slots);
+  p.moves = int(moves);
   p.counts = counts;
   p.new_lens = new_lens;
   p.vec = ((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(positions)) % 16 ==

@@ -11,7 +11,7 @@ import torch
 from bpt import BptArgumentError, _lib, diff
 from test_evict_cpu import decode_args, scored, tensors
 
-c_vp = ctypes.c_void_p
+c_i32, c_i64, c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 FLOAT_MAX = torch.finfo(torch.float32).max
 
 
@@ -87,3 +87,39 @@ def test_abi_numbers(status, kw):
     rc = _lib.lib().bpt_decode_scored(ctypes.byref(decode_args(**kw)), c_vp(0x200000),
                                       ctypes.c_size_t(16), None)
     assert rc == status
+
+
+# B=3, 2 kv heads, 32 slots, budget 8: 6 rows of 8 moves. Addresses of non-overlapping arrays.
+SELECT = dict(scores=0x100000, positions=0x110000, seq_lens=0x120000, next_pos=0x121000,
+              src=0x130000, dst=0x131000, counts=0x132000, new_lens=0x133000)
+
+
+def select_rc(batch=3, pos_sb=64, pos_sh=32, **kw):
+    """bpt_select_evictions at these addresses, refused before a launch in every case used here."""
+    a = {k: c_vp(v) for k, v in {**SELECT, **kw}.items()}
+    return _lib.lib().bpt_select_evictions(
+        a["scores"], c_i64(64), c_i64(32), a["positions"], c_i64(pos_sb), c_i64(pos_sh),
+        a["seq_lens"], a["next_pos"], c_i32(batch), c_i32(2), c_i32(32), c_i32(8), c_i32(0),
+        c_i32(0), a["src"], a["dst"], a["counts"], a["new_lens"], None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(new_lens=SELECT["next_pos"]), dict(new_lens=SELECT["next_pos"] + 8),
+    dict(new_lens=SELECT["seq_lens"] - 8), dict(new_lens=SELECT["seq_lens"]),
+    dict(counts=SELECT["seq_lens"] - 20), dict(src=SELECT["next_pos"] - 4 * 47),
+    dict(dst=SELECT["seq_lens"]), dict(dst=SELECT["src"] + 4 * 47),
+    dict(counts=SELECT["new_lens"] - 20), dict(src=SELECT["scores"] + 4 * 191),
+    dict(src=SELECT["positions"] - 4 * 47),
+    dict(dst=SELECT["positions"] - 4 * 128, pos_sb=-64)])
+def test_abi_select_results_on_inputs(kw):
+    """One CTA writes new_lens and the moves that others of the row have still to read the inputs
+    of: overlapping arrays are refused, shifted ones too."""
+    assert select_rc(**kw) == _lib.ERR_INVALID_ARGUMENT
+
+
+def test_abi_select_neighbours_are_no_overlap():
+    """Arrays that touch pass the check: with 2^26 sequences the next refusal is the grid's size."""
+    far = {k: i << 40 for i, k in enumerate(SELECT, 1)}
+    end = far["src"] + 4 * (1 << 27) * 8
+    assert select_rc(batch=1 << 26, **{**far, "dst": end}) == _lib.ERR_UNSUPPORTED_SHAPE
+    assert select_rc(batch=1 << 26, **{**far, "dst": end - 4}) == _lib.ERR_INVALID_ARGUMENT
