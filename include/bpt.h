@@ -44,7 +44,8 @@ enum bpt_device_flags {
   BPT_DEV_BAD_BLOCK_ID = 1,    /* block_table entry outside [0, num_blocks) */
   BPT_DEV_SEQ_TOO_LONG = 2,    /* seq_len > max_blocks * block_size (clamped) */
   BPT_DEV_WAIT_TIMEOUT = 4,    /* a pipeline wait gave up after its time budget */
-  BPT_DEV_NEG_SEQ_LEN = 8      /* seq_len < 0 (treated as 0) */
+  BPT_DEV_NEG_SEQ_LEN = 8,     /* seq_len < 0 (treated as 0) */
+  BPT_DEV_BAD_NEW_LEN = 16     /* new_len outside [0, max_new] (clamped) */
 };
 
 const char* bpt_status_string(int status);
@@ -251,7 +252,7 @@ typedef struct bpt_paged_cache {
  * token, head) to slots seq_lens[b] + t. Where given, scores of the new slots become 0 and
  * positions next_pos[b] + t, for v_heads heads (T >= max_blocks * block_size). Tokens past the
  * table, and tokens of a page outside the cache, are not written and flagged in *status
- * (nullable). Nothing else is touched: the caller advances seq_lens. */
+ * (nullable); new_lens outside [0, max_new] are clamped to it and flagged. Nothing else is touched: the caller advances seq_lens. */
 int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new, const int64_t* kn_stride,
                       const void* v_new, const int64_t* vn_stride, const int32_t* new_lens,
                       const int32_t* seq_lens, const int32_t* block_table, int64_t bt_sb,

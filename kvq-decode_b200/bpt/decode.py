@@ -27,7 +27,8 @@ CHECKS = os.environ.get("BPT_CHECKS", "0") not in ("", "0")
 DEVICE_FLAGS = {1: "block_table entry outside [0, num_blocks)",
                 2: "seq_len > max_blocks * block_size",
                 4: "pipeline wait timed out",
-                8: "negative seq_len"}
+                8: "negative seq_len",
+                16: "new_lens entry outside [0, number of new tokens]"}
 
 
 @functools.lru_cache(maxsize=None)

@@ -138,8 +138,9 @@ def append_tokens(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Ten
 
     scores of the new slots become 0 and positions next_pos[b] + t where those are given. The
     heads are those of each cache, so a differential cache (``bpt.diff``) is appended to with the
-    same call. Tokens past the block table are not written (checked mode raises). seq_lens
-    is not changed: the caller advances it. Runs on the current stream, no host synchronisation.
+    same call. Tokens past the block table are not written, and new_lens are clamped to [0, S]
+    (checked mode raises on both). seq_lens is not changed: the caller advances it, by no more than
+    was written. Runs on the current stream, no host synchronisation.
     """
     status = _status(k_cache)
     (_BIND or _bind()).append_tokens(k_cache, v_cache, k_new, v_new, new_lens, seq_lens,

@@ -539,6 +539,9 @@ append_kernel(const AppendParams p) {
   const int b = blockIdx.z;
   const int new_len = p.new_lens[b], start = p.seq_lens[b];
   const int m = min(max(new_len, 0), p.max_new), t0 = int(blockIdx.x) * U;
+  // one thread a sequence, and before the CTAs without tokens leave
+  if (new_len != m && (blockIdx.x | blockIdx.y | threadIdx.x) == 0)
+    flag_device_error(p.status, BPT_DEV_BAD_NEW_LEN);
   if (t0 >= m) return;
   const int kw = p.k.row_bytes / W, vw = p.v.row_bytes / W;
   const int k_items = p.k_heads * kw, items = k_items + p.v_heads * vw;
@@ -804,8 +807,9 @@ extern "C" int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new
   if (!cache || bad_cache(*cache) || batch < 0 || max_new < 0 || max_blocks < 0)
     return BPT_ERR_INVALID_ARGUMENT;
   if (bad_pages(*cache)) return BPT_ERR_UNSUPPORTED_SHAPE;
-  if (batch == 0 || max_new == 0) return BPT_OK;
-  if (!k_new || !v_new || !kn_stride || !vn_stride || !new_lens || !seq_lens ||
+  // with no rows there is nothing to write, but lengths that ask for some are flagged
+  if (batch == 0 || (max_new == 0 && !status)) return BPT_OK;
+  if ((max_new > 0 && (!k_new || !v_new)) || !kn_stride || !vn_stride || !new_lens || !seq_lens ||
       (!block_table && max_blocks > 0) || (positions && !next_pos))
     return BPT_ERR_INVALID_ARGUMENT;
   AppendParams p{};
@@ -839,7 +843,7 @@ extern "C" int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new
   const int64_t blocks = (items + kAppendThreads - 1) / kAppendThreads;
   if (blocks > kMaxGridYZ || batch > kMaxGridYZ) return BPT_ERR_UNSUPPORTED_SHAPE;
   const int U = max_new == 1 ? 1 : kPromptTokens;
-  const dim3 grid(max_new / U + (max_new % U != 0), unsigned(blocks), batch);
+  const dim3 grid(max_new > 0 ? max_new / U + (max_new % U != 0) : 1, unsigned(blocks), batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto kern = vec ? (U == 1 ? append_kernel<uint4, 1> : append_kernel<uint4, kPromptTokens>)
                   : (U == 1 ? append_kernel<uint16_t, 1>
