@@ -33,6 +33,7 @@ that is appended to or evicted must own its pages alone. ``bpt.diff`` has the di
 over such a cache.
 """
 import ctypes
+import importlib
 from typing import NamedTuple, Optional
 
 import torch
@@ -52,10 +53,13 @@ def _bind():
     if _BIND is None:
         lib = _lib.lib()
         try:
-            from . import _bind as module
-        except ImportError as e:
+            module = importlib.import_module("._bind", __package__)
+        except ModuleNotFoundError as e:
             raise ImportError("bpt/_bind is not built; build it with `python "
                               "kvq-decode_b200/build.py` (there is no fallback)") from e
+        except ImportError as e:
+            raise ImportError(f"bpt/_bind does not load ({e}); rebuild it for this torch with "
+                              "`python kvq-decode_b200/build.py`") from e
         module.init({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _ABI},
                     _lib.BptArgumentError, _lib.check)
         _BIND = module

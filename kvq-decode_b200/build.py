@@ -8,10 +8,12 @@ with nvcc and links one shared library exporting the C ABI declared in ``include
 ``bpt/_bind`` (the Python binding of the scored decode and the eviction).
 The CUDA runtime is linked statically; the driver API is reached through
 ``cudaGetDriverEntryPointByVersion`` so the library has no link-time libcuda dependency.
-Rebuilds only when a source or header is newer than what was built.
+Rebuilds only when a source or header is newer than what was built, or torch (whose C++ ABI
+``bpt/_bind`` is tied to) is another than it was built with.
 """
 import argparse
 import glob
+import importlib.metadata
 import os
 import shutil
 import subprocess
@@ -24,6 +26,7 @@ CSRC = os.path.join(PKG, "csrc")
 OUT = os.path.join(PKG, "bpt", "libbpt_b200.so")
 BIND_SRC = os.path.join(CSRC, "bind.cpp")
 BIND_OUT = os.path.join(PKG, "bpt", "_bind" + sysconfig.get_config_var("EXT_SUFFIX"))
+BIND_STAMP = os.path.join(PKG, "_build", "bind.torch")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr",
          "-Xptxas", "-O3"]
@@ -58,9 +61,17 @@ def up_to_date() -> bool:
     return newer(OUT, deps())
 
 
+def bind_built_for() -> str:
+    """The torch whose C++ ABI ``bpt/_bind`` is tied to."""
+    return f"torch {importlib.metadata.version('torch')}\n"
+
+
 def bind_up_to_date() -> bool:
-    return newer(BIND_OUT, [BIND_SRC, os.path.join(ROOT, "include", "bpt.h"),
-                            os.path.abspath(__file__)])
+    if not newer(BIND_OUT, [BIND_SRC, os.path.join(ROOT, "include", "bpt.h"),
+                            os.path.abspath(__file__)]) or not os.path.exists(BIND_STAMP):
+        return False
+    with open(BIND_STAMP) as f:
+        return f.read() == bind_built_for()
 
 
 def start_bind(verbose: bool):
@@ -90,6 +101,9 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> str:
         if bind.returncode != 0:
             raise RuntimeError(f"{BIND_SRC} failed:\n{out}")
         os.replace(BIND_OUT + ".tmp", BIND_OUT)
+        os.makedirs(os.path.dirname(BIND_STAMP), exist_ok=True)
+        with open(BIND_STAMP, "w") as f:
+            f.write(bind_built_for())
     return OUT
 
 
