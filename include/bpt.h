@@ -269,7 +269,8 @@ int bpt_evict_moves(int budget, int slots);
  * receive the moves that bring them to slots < budget: the i-th evicted slot below budget, in
  * ascending order, takes the i-th kept slot at or past it, in descending order; -1 past
  * counts[b, h]. new_lens[b] = min(seq_lens[b], budget). src, dst, counts and new_lens may not
- * overlap an input or one another. Lengths are clamped to [0, slots]. Needs recent + sinks <= budget. */
+ * overlap an input or one another. Lengths are clamped to [0, slots]. Needs recent + sinks <=
+ * budget and fewer than 2^31 - 16384 slots. */
 int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t sc_sh,
                          const int32_t* positions, int64_t pos_sb, int64_t pos_sh,
                          const int32_t* seq_lens, const int32_t* next_pos, int batch,

@@ -421,7 +421,8 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   // the caches
   if (misaligned(a->q, 4) || a->q_stride[0] % 2 || a->q_stride[1] % 2) return BPT_ERR_ALIGNMENT;
   const int64_t cap = int64_t(a->max_blocks) * a->block_size;
-  if (cap > INT32_MAX) return BPT_ERR_UNSUPPORTED_SHAPE;
+  // the ends of the last chunk's tokens are ints
+  if (cap > INT32_MAX - kChunk) return BPT_ERR_UNSUPPORTED_SHAPE;
   const int S = state_splits(width, a->batch, a->kv_heads, a->block_size, a->max_blocks,
                              a->num_splits, a->sm_count);
   const int64_t tokens = a->scores ? cap : 0;

@@ -601,6 +601,12 @@ append_kernel(const AppendParams p) {
 }
 
 constexpr int kMaxGridYZ = 65535;
+// Slots and moves are ints, and so are the ends of the last slice, tile or warp's moves, which pass
+// them by less than this.
+constexpr int kIndexRoom = 16384;
+static_assert(kIndexRoom > 2 * kMaxCluster * kTile + 2 * kSelWarps * kTile &&
+                  kIndexRoom > 32 * kMoveWarps,
+              "slices and warps are rounded up to whole tiles");
 
 int log2_of(int x) {
   int s = 0;
@@ -697,7 +703,8 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   for (int i = 0; i < 4; ++i)
     for (int j = i + 1; j < 8; ++j)
       if (range[i].meets(range[j])) return BPT_ERR_INVALID_ARGUMENT;
-  if (rows > INT32_MAX / kMaxCluster) return BPT_ERR_UNSUPPORTED_SHAPE;
+  if (rows > INT32_MAX / kMaxCluster || slots > INT32_MAX - kIndexRoom)
+    return BPT_ERR_UNSUPPORTED_SHAPE;
   const int C = cluster_size(rows, slots, device_sm_count());
   SelectParams p{};
   p.scores = scores;
@@ -756,7 +763,7 @@ extern "C" int bpt_compact_cache(const bpt_paged_cache* cache, const int32_t* bl
   if (!cache || bad_cache(*cache) || batch < 0 || moves < 0 || max_blocks < 0 || slots < 0)
     return BPT_ERR_INVALID_ARGUMENT;
   if (cache->k_heads != cache->v_heads) return BPT_ERR_INVALID_ARGUMENT;
-  if (bad_pages(*cache)) return BPT_ERR_UNSUPPORTED_SHAPE;
+  if (bad_pages(*cache) || moves > INT32_MAX - kIndexRoom) return BPT_ERR_UNSUPPORTED_SHAPE;
   if (batch == 0 || moves == 0) return BPT_OK;
   if ((!block_table && max_blocks > 0) || !src || !dst || !counts) return BPT_ERR_INVALID_ARGUMENT;
   CompactParams p{};

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from bpt import BptArgumentError, _lib, diff
-from test_evict_cpu import decode_args, scored, tensors
+from test_evict_cpu import cache_args, decode_args, scored, tensors
 
 c_i32, c_i64, c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 FLOAT_MAX = torch.finfo(torch.float32).max
@@ -94,12 +94,12 @@ SELECT = dict(scores=0x100000, positions=0x110000, seq_lens=0x120000, next_pos=0
               src=0x130000, dst=0x131000, counts=0x132000, new_lens=0x133000)
 
 
-def select_rc(batch=3, pos_sb=64, pos_sh=32, **kw):
+def select_rc(batch=3, slots=32, pos_sb=64, pos_sh=32, **kw):
     """bpt_select_evictions at these addresses, refused before a launch in every case used here."""
     a = {k: c_vp(v) for k, v in {**SELECT, **kw}.items()}
     return _lib.lib().bpt_select_evictions(
         a["scores"], c_i64(64), c_i64(32), a["positions"], c_i64(pos_sb), c_i64(pos_sh),
-        a["seq_lens"], a["next_pos"], c_i32(batch), c_i32(2), c_i32(32), c_i32(8), c_i32(0),
+        a["seq_lens"], a["next_pos"], c_i32(batch), c_i32(2), c_i32(slots), c_i32(8), c_i32(0),
         c_i32(0), a["src"], a["dst"], a["counts"], a["new_lens"], None)
 
 
@@ -123,3 +123,33 @@ def test_abi_select_neighbours_are_no_overlap():
     end = far["src"] + 4 * (1 << 27) * 8
     assert select_rc(batch=1 << 26, **{**far, "dst": end}) == _lib.ERR_UNSUPPORTED_SHAPE
     assert select_rc(batch=1 << 26, **{**far, "dst": end - 4}) == _lib.ERR_INVALID_ARGUMENT
+
+
+INT32_MAX = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("bs,max_blocks,status", [
+    (16, INT32_MAX // 16, _lib.ERR_UNSUPPORTED_SHAPE),          # 2^31 - 16 slots
+    (32, INT32_MAX // 32, _lib.ERR_UNSUPPORTED_SHAPE),
+    (16, INT32_MAX // 16 - 2, _lib.ERR_WORKSPACE_TOO_SMALL)])
+def test_abi_decode_next_to_2_31_slots(bs, max_blocks, status):
+    """The last chunk's end has to be an int too."""
+    a = decode_args(block_size=bs, max_blocks=max_blocks)
+    assert _lib.lib().bpt_decode_scored(ctypes.byref(a), c_vp(0x200000), ctypes.c_size_t(16),
+                                        None) == status
+
+
+@pytest.mark.parametrize("slots", [INT32_MAX, INT32_MAX - 2000])
+def test_abi_select_next_to_2_31_slots(slots):
+    """A cluster's last slice ends up to 16 tiles past the row: refused where that passes an int."""
+    far = {k: i << 40 for i, k in enumerate(SELECT, 1)}
+    assert select_rc(slots=slots, **far) == _lib.ERR_UNSUPPORTED_SHAPE
+
+
+@pytest.mark.parametrize("moves", [INT32_MAX, INT32_MAX - 100])
+def test_abi_compact_next_to_2_31_moves(moves):
+    c, p = cache_args(), c_vp(0x300000)
+    rc = _lib.lib().bpt_compact_cache(
+        ctypes.byref(c), p, c_i64(2), c_i32(2), p, p, p, c_i32(moves), c_i32(1), None, c_i64(0),
+        c_i64(0), None, c_i64(0), c_i64(0), c_i32(32), None, None)
+    assert rc == _lib.ERR_UNSUPPORTED_SHAPE
