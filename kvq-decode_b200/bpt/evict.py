@@ -105,7 +105,7 @@ def scored_workspace_bytes(q: torch.Tensor, k_cache: torch.Tensor, block_table: 
                            scored: bool = True) -> int:
     """Bytes of a ``workspace`` for a decode of these shapes (maps 2: the differential one). A
     workspace serves calls that follow one another on a stream, captured ones among them; two
-    calls that may run at the same time need one each."""
+    calls that may run at the same time need one each. A call given less allocates its own."""
     return _bind().scored_workspace_bytes(maps, q, k_cache, block_table, num_splits or 0, scored)
 
 
@@ -158,11 +158,12 @@ def select_evictions(scores: torch.Tensor, positions: torch.Tensor, seq_lens: to
                      moves: Optional[EvictionMoves] = None) -> EvictionMoves:
     """Choose the ``budget`` tokens that each kv head of each sequence keeps -> EvictionMoves.
 
-    A sequence of at most budget tokens keeps all. Otherwise the tokens of position < sinks or
-    >= next_pos - recent are kept (recent + sinks <= budget), then those of the highest score,
-    ties and NaN (below every number) by the lowest slot. The moves bring them to slots 0 ..
-    budget - 1: the i-th evicted slot below budget takes the i-th kept slot from the end. Nothing is
-    moved yet; ``compact_cache`` does that. ``moves`` reuses the tensors of an earlier result.
+    Lengths count as at most the rows' width T. A sequence of at most budget tokens keeps all.
+    Otherwise the tokens of position < sinks or >= next_pos - recent are kept (recent + sinks <=
+    budget), then those of the highest score, ties and NaN (below every number) by the lowest slot.
+    The moves bring them to slots 0 .. budget - 1: the i-th evicted slot below budget takes the i-th
+    kept slot from the end. Nothing is moved yet; ``compact_cache`` does that. ``moves`` reuses the
+    tensors of an earlier result.
     """
     return EvictionMoves._make((_BIND or _bind()).select_evictions(
         scores, positions, seq_lens, next_pos, budget, recent, sinks, moves))

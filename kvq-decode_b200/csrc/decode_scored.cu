@@ -36,13 +36,16 @@ constexpr int kFinishThreads = kFinishWarps * 32;
 constexpr int kScoreTokens = 4 * kFinishThreads;  // tokens of a round of a scoring CTA
 constexpr int kMaxRows = 8;                       // q rows per kv head
 static_assert(kMaxRows >= kFinishWarps, "shared rows double as one value a warp");
-// Scoring CTAs an SM, as many as fit at once, each of several rounds: 29 us for 59 MB of logits
-// with a CTA per 1024 tokens (B=16, 24-32k tokens, 32 q heads), 20 us with 3 or 4 an SM; the whole
-// call at B=8, 12-16k tokens 81.4 us with 3 (two rounds), 82.4 with 4 and more (one).
+// A scoring CTA takes a further round of tokens for every kScoreCtas CTAs an SM that one round each
+// would need: at least kScoreCtas and less than twice as many an SM are launched (the rounding of a
+// row's parts aside). 29 us for 59 MB of logits with a CTA per 1024 tokens (4096 CTAs: B=16, 24-32k
+// tokens, 32 q heads), 20 us with 512 or 768; the whole call at B=8, 12-16k tokens 81.4 us with 512
+// CTAs of two rounds (3), 82.4 with 1024 of one (4 and more).
 constexpr int kScoreCtas = 3;
 // The logits stay in L2 (evict-last stores). A buffer that would be written back while the next
 // call streams its cache is dropped line by line once read: 306 -> 298 us at 59 MB, 627 -> 620
-// at 114 MB (B=16). At 17 MB dropping costs more than it saves: 89 -> 92 us (B=1, 128k tokens).
+// at 114 MB (B=16). At 17 MB dropping costs more than it saves: 89 -> 92 us (B=1, 128k tokens), the
+// call alone. Smaller buffers so outlive the call in L2 at raised priority, up to a quarter of it.
 constexpr int64_t kDropBytes = 32 << 20;
 
 // Split CTA shape: 2 warps of 16 tokens each, and as many stages and CTAs an SM as keep about
@@ -497,7 +500,7 @@ extern "C" int bpt_decode_scored(const bpt_scored_decode* a, void* workspace,
   f.splits = S;
   f.out_heads = a->q_heads / maps;
   f.n_merge = a->batch * f.out_heads;
-  // rounds: one while the CTAs fit the SMs at once, then what keeps them to kScoreCtas an SM
+  // rounds: one below 2 * kScoreCtas CTAs an SM, then what keeps them below that (floor)
   const int64_t steps = (cap + kScoreTokens - 1) / kScoreTokens;
   const int64_t rows = int64_t(a->batch) * a->kv_heads;
   const int64_t most = int64_t(kScoreCtas) * device_sm_count();

@@ -156,7 +156,7 @@ __device__ __forceinline__ void split_hi_lo(float p0, float p1, uint32_t& hi, ui
 }
 
 // p = hi + mid + lo in bf16 (a bf16 MMA takes no other operand), exactly: each remainder is exact,
-// and 3 x 8 bits hold fp32's 24. Two limbs (a relative error of up to 2^-17) put 1 in 200 outputs of
+// and 3 x 8 bits hold fp32's 24. Two limbs (a relative error of up to 2^-17) put 1 in 300 outputs of
 // a normalised differential layer one bf16 step beside what fp32 weights give.
 __device__ __forceinline__ void split_bf16(float p0, float p1, uint32_t& hi, uint32_t& mid,
                                            uint32_t& lo) {
@@ -268,6 +268,8 @@ split_kv_fp16_mma_kernel(const __grid_constant__ CUtensorMap tmK,
     // -> 8.1, 11.5 -> 9.8 us), and throughout where boxes are many or small (B=8, 0.47 GB: 130 ->
     // 89 us at 64 channels, 92 -> 81 us at 256 channels in pages of 16). Elsewhere the paced stream
     // of one lane is 2 % faster (B=4, 64k tokens of 128 channels: 174 against 178 us): it stays.
+    // The first chunks' rule costs long splits of large boxes a little: 82.3 -> 83.0 us (B=8, 12-16k
+    // tokens, differential of 256 channels in pages of 32).
     static_assert(!Op::kState || (CHUNK / 16) * 2 * C::NCB <= 32, "a lane per box of a chunk");
     bool many_boxes = CHUNK / R * C::NCB >= 8;
     if (D == 64) many_boxes = true;
