@@ -207,7 +207,8 @@ enum bpt_dtype { BPT_FP16 = 1, BPT_BF16 = 2 };
  *   [.., Hkv, 2 D], out [B, H, 2 D]; H / Hkv <= 4; D 64 or 128. q_heads is 2 H. Output head j is
  *   (softmax(q_2j.k_2h) - lam_j softmax(q_2j+1.k_2h+1)) v_h, h = j / (H / Hkv); where norm_weight
  *   [2 D] is set it is divided by sqrt(mean square + norm_eps) and multiplied by the weight (a
- *   row whose fp32 mean square is 0 gives zeros, norm_eps 0 included); then by out_scale. The score adds the sum of |weight of map 1 - lam_j weight of map 2|.
+ *   row whose fp32 mean square is 0 gives zeros, norm_eps 0 included); then by out_scale. The
+ *   score adds the sum of |weight of map 1 - lam_j weight of map 2|.
  * q, caches and out are fp16 or bf16; scores, lam and norm_weight fp32. Softmax, sums and
  * scores are fp32. An empty sequence gives zeros. decay 0 ignores the old scores (NaN among
  * them); slots past a sequence's end keep theirs. Keys must be finite with maps 2. */
@@ -252,7 +253,8 @@ typedef struct bpt_paged_cache {
  * token, head) to slots seq_lens[b] + t. Where given, scores of the new slots become 0 and
  * positions next_pos[b] + t, for v_heads heads (T >= max_blocks * block_size). Tokens past the
  * table, and tokens of a page outside the cache, are not written and flagged in *status
- * (nullable); new_lens outside [0, max_new] are clamped to it and flagged. Nothing else is touched: the caller advances seq_lens. */
+ * (nullable); new_lens outside [0, max_new] are clamped to it and flagged. Nothing else is
+ * touched: the caller advances seq_lens. */
 int bpt_append_tokens(const bpt_paged_cache* cache, const void* k_new, const int64_t* kn_stride,
                       const void* v_new, const int64_t* vn_stride, const int32_t* new_lens,
                       const int32_t* seq_lens, const int32_t* block_table, int64_t bt_sb,

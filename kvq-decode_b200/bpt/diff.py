@@ -47,7 +47,8 @@ def paged_decode_attention_diff(q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     D 64 or 128, at most 4 output heads per value head; keys must be finite. lam is fp32 [H], or
     [B, H] where it depends on the token. norm_weight fp32 [2 D]: o / sqrt(mean(o^2) + norm_eps) *
     norm_weight, zeros where the mean is 0 (norm_eps may be 0); the result is then multiplied by
-    out_scale. Softmax, sums and the norm are fp32, rounded once. With ``scores`` [B, Hkv, T] fp32 (``bpt.evict``), slot t of value head h gets
+    out_scale. Softmax, sums and the norm are fp32, rounded once. With ``scores`` [B, Hkv, T] fp32
+    (``bpt.evict``), slot t of value head h gets
 
         scores[b, h, t] = decay * scores[b, h, t] + sum_j |map-1 weight - lam_j * map-2 weight|
 

@@ -643,13 +643,20 @@ Range words(const void* p, int64_t n) {
   return {a, a + uintptr_t(n) * 4};
 }
 
-// What rows [batch, heads, slots] of state can reach.
-Range state_words(const void* p, int64_t sb, int64_t sh, int batch, int heads, int slots) {
-  if (!p || slots == 0) return {0, 0};
-  const int64_t b = sb * (batch - 1), h = sh * (heads - 1);
+// Whether r meets a row of state [batch, heads, slots]. Rows are looked at one by one only where r
+// lies between the first and the last of them.
+bool meets_rows(const Range& r, const void* p, int64_t sb, int64_t sh, int batch, int heads,
+                int slots) {
+  if (slots == 0) return false;
   const char* base = static_cast<const char*>(p);
-  return {reinterpret_cast<uintptr_t>(base + 4 * ((b < 0 ? b : 0) + (h < 0 ? h : 0))),
-          reinterpret_cast<uintptr_t>(base + 4 * ((b > 0 ? b : 0) + (h > 0 ? h : 0) + slots))};
+  const int64_t b1 = 4 * sb * (batch - 1), h1 = 4 * sh * (heads - 1);
+  const char* low = base + (b1 < 0 ? b1 : 0) + (h1 < 0 ? h1 : 0);
+  const char* high = base + (b1 > 0 ? b1 : 0) + (h1 > 0 ? h1 : 0);
+  if (!r.meets({reinterpret_cast<uintptr_t>(low), words(high, slots).hi})) return false;
+  for (int b = 0; b < batch; ++b)
+    for (int h = 0; h < heads; ++h)
+      if (r.meets(words(base + 4 * (b * sb + h * sh), slots))) return true;
+  return false;
 }
 
 bool vec16(const CacheView& v) {
@@ -696,13 +703,15 @@ extern "C" int bpt_select_evictions(const float* scores, int64_t sc_sb, int64_t 
   // one CTA writes what others of the row have still to read: no result may lie on an input, nor
   // on another result
   const int64_t moves = bpt_evict_moves(budget, slots);
-  const Range range[8] = {words(src, rows * moves), words(dst, rows * moves), words(counts, rows),
-                          words(new_lens, batch), words(seq_lens, batch), words(next_pos, batch),
-                          state_words(scores, sc_sb, sc_sh, batch, kv_heads, slots),
-                          state_words(positions, pos_sb, pos_sh, batch, kv_heads, slots)};
-  for (int i = 0; i < 4; ++i)
-    for (int j = i + 1; j < 8; ++j)
+  const Range range[6] = {words(src, rows * moves), words(dst, rows * moves), words(counts, rows),
+                          words(new_lens, batch), words(seq_lens, batch), words(next_pos, batch)};
+  for (int i = 0; i < 4; ++i) {
+    for (int j = i + 1; j < 6; ++j)
       if (range[i].meets(range[j])) return BPT_ERR_INVALID_ARGUMENT;
+    if (meets_rows(range[i], scores, sc_sb, sc_sh, batch, kv_heads, slots) ||
+        meets_rows(range[i], positions, pos_sb, pos_sh, batch, kv_heads, slots))
+      return BPT_ERR_INVALID_ARGUMENT;
+  }
   if (rows > INT32_MAX / kMaxCluster || slots > INT32_MAX - kIndexRoom)
     return BPT_ERR_UNSUPPORTED_SHAPE;
   const int C = cluster_size(rows, slots, device_sm_count());

@@ -157,7 +157,9 @@ __device__ __forceinline__ void split_hi_lo(float p0, float p1, uint32_t& hi, ui
 
 // p = hi + mid + lo in bf16 (a bf16 MMA takes no other operand), exactly: each remainder is exact,
 // and 3 x 8 bits hold fp32's 24. Two limbs (a relative error of up to 2^-17) put 1 in 300 outputs of
-// a normalised differential layer one bf16 step beside what fp32 weights give.
+// a normalised differential layer one bf16 step beside what fp32 weights give. The third costs one
+// product more: B=8, 12-16k tokens, 82.0 -> 82.5 us at 128 channels and 4 rows, 89.8 -> 90.1 at 8
+// rows, 81.1 -> 83.0 and 86.9 -> 93.6 at 256 channels.
 __device__ __forceinline__ void split_bf16(float p0, float p1, uint32_t& hi, uint32_t& mid,
                                            uint32_t& lo) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(p0, p1);

@@ -128,6 +128,18 @@ def test_abi_select_neighbours_are_no_overlap():
 INT32_MAX = 2 ** 31 - 1
 
 
+@pytest.mark.parametrize("word,status", [
+    (INT32_MAX, _lib.ERR_UNSUPPORTED_SHAPE), (INT32_MAX - 1, _lib.ERR_INVALID_ARGUMENT),
+    ((1 << 34) - 3, _lib.ERR_UNSUPPORTED_SHAPE), ((1 << 34) - 2, _lib.ERR_INVALID_ARGUMENT),
+    (5 << 33, _lib.ERR_UNSUPPORTED_SHAPE), ((1 << 37) + (1 << 34) + 5, _lib.ERR_INVALID_ARGUMENT)])
+def test_abi_select_results_between_rows(word, status):
+    """new_lens (3 words) in the room between two rows of positions is no overlap, and on a row it is.
+    Rows of 2^31 - 1 slots, 2^34 words apart: what passes is refused for that length afterwards."""
+    far = {k: i << 50 for i, k in enumerate(SELECT, 1)}
+    far["new_lens"] = far["positions"] + 4 * word
+    assert select_rc(slots=INT32_MAX, pos_sb=1 << 36, pos_sh=1 << 34, **far) == status
+
+
 @pytest.mark.parametrize("bs,max_blocks,status", [
     (16, INT32_MAX // 16, _lib.ERR_UNSUPPORTED_SHAPE),          # 2^31 - 16 slots
     (32, INT32_MAX // 32, _lib.ERR_UNSUPPORTED_SHAPE),
